@@ -406,6 +406,73 @@ int mvr_regularize_normalize_views_backward(const float *grad_out, int32_t n_ima
                                             const int32_t *crop_j, int32_t pad, const float *mean, const float *std_,
                                             float *grad_images, mvr_stream_t stream);
 
+/* ---- the tokens of rendered views: what a network over the views' patches does with them next ----
+ *
+ * Operators of their own, not of the reference: a token's place is its view's camera and its patch, a view dropped by the
+ * regulariser (scale 0, above) is left out.  Element types of the tensors: */
+enum {
+  MVR_TYPE_FLOAT = 0,  /* 32 bits */
+  MVR_TYPE_HALF = 1,   /* IEEE 16 bits */
+  MVR_TYPE_BFLOAT = 2  /* bfloat16 */
+};
+
+/* Rotary positions with several axes: pair i of a head, which belongs to axis a(i), turns by 2 pi positions[a(i)] turns[i]:
+ *   out1 = x1 cos - x2 sin,  out2 = x1 sin + x2 cos
+ * pairs are (i, i + n), or (2 i, 2 i + 1) when `interleaved`; n = the sections' sum; the rest of a head is copied.
+ * Angles are formed and reduced in 64 bits, so far positions (1e6 and more) keep 32-bit accuracy. */
+typedef struct mvr_rotary_params {
+  int32_t batch, tokens, heads, dim;   /* dim <= 256 */
+  int32_t type;                        /* MVR_TYPE_* of x, out and their gradients */
+  int32_t axes;                        /* 1..4 */
+  int32_t sections[4];                 /* pairs of each axis, in order; 2 * sum <= dim */
+  int32_t interleaved;
+  int32_t reserved_;                   /* explicit padding; must be 0 */
+  int64_t x_stride[3];                 /* of x, in elements: batch, token, head; a head's elements are contiguous */
+  int64_t grad_stride[3];              /* of grad_out, the same (backward only) */
+  int64_t position_stride[2];          /* of positions: batch (0: shared), token; a token's axes are contiguous */
+} mvr_rotary_params;
+
+/* turns: HOST doubles, one per pair: turns per unit of position.  positions: (batch, tokens, axes) f32 by its strides.
+ * out: (batch, tokens, heads, dim) contiguous, not x. */
+int mvr_rotate_tokens_forward(const mvr_rotary_params *params, const double *turns, const void *x, const float *positions,
+                              void *out, mvr_stream_t stream);
+/* grad_x: contiguous.  grad_positions (batch, tokens, axes) f32 contiguous and x go together, or both are NULL.  Sums are
+ * taken in a fixed order (bit-reproducible). */
+int mvr_rotate_tokens_backward(const mvr_rotary_params *params, const double *turns, const void *x, const float *positions,
+                               const void *grad_out, void *grad_x, float *grad_positions, mvr_stream_t stream);
+
+/* The end of one block and the norm in front of the next, over rows of `dim` elements:
+ *   n = post_weight * N(branch)   (branch itself where post_weight is NULL)
+ *   y = residual + s * gate * n
+ *   z = N(y) * weight + bias
+ * N divides a row by sqrt(mean square + eps); kind 1 (layer) takes the row's mean off first. */
+typedef struct mvr_norm_params {
+  int64_t rows;
+  int32_t dim;             /* <= 8192 */
+  int32_t residual_type;   /* of residual, y and their gradients: the branch's type, or 32 bits */
+  int32_t branch_type;     /* of branch, z and their gradients */
+  int32_t param_type;      /* of weight, bias, post_weight, gate and their gradients */
+  int32_t kind;            /* 0: rms, 1: layer */
+  int32_t reserved_;       /* explicit padding; must be 0 */
+  int64_t gate_groups;     /* gate: (gate_groups, dim), each for rows / gate_groups consecutive rows; 0: no gate */
+  int64_t scale_groups;    /* scale: (scale_groups) f32, the same; 0: the number below for every row */
+  float scale, eps;
+} mvr_norm_params;
+
+/* All tensors contiguous.  A row whose `scale` is 0 (a dropped view) keeps its residual; its branch is not read.
+ * stats: (rows, 4) f32 for the backward, or NULL.  y may be residual itself. */
+int mvr_add_norm_tokens_forward(const mvr_norm_params *params, const void *residual, const void *branch, const void *weight,
+                                const void *bias, const void *post_weight, const void *gate, const float *scale, void *y,
+                                void *z, float *stats, mvr_stream_t stream);
+size_t mvr_add_norm_tokens_workspace_bytes(const mvr_norm_params *params);
+/* grad_y or grad_z may be NULL (zero), the parameters' gradients may each be NULL (not wanted).  The workspace is needed for
+ * the latter; sums are taken in a fixed order (bit-reproducible). */
+int mvr_add_norm_tokens_backward(const mvr_norm_params *params, const void *y, const void *branch, const void *weight,
+                                 const void *post_weight, const void *gate, const float *scale, const float *stats,
+                                 const void *grad_y, const void *grad_z, void *grad_residual, void *grad_branch,
+                                 void *grad_weight, void *grad_bias, void *grad_post_weight, void *grad_gate,
+                                 void *workspace, size_t workspace_bytes, mvr_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

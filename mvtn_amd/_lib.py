@@ -61,10 +61,29 @@ class PackLayout(ctypes.Structure):  # struct mvr_pack_layout
                 ("face_off_at", ctypes.c_uint64), ("bytes", ctypes.c_uint64)]
 
 
+class RotaryParams(ctypes.Structure):  # struct mvr_rotary_params
+    _fields_ = [("batch", ctypes.c_int32), ("tokens", ctypes.c_int32), ("heads", ctypes.c_int32), ("dim", ctypes.c_int32),
+                ("type", ctypes.c_int32), ("axes", ctypes.c_int32), ("sections", ctypes.c_int32 * 4), ("interleaved", ctypes.c_int32),
+                ("reserved_", ctypes.c_int32), ("x_stride", ctypes.c_int64 * 3), ("grad_stride", ctypes.c_int64 * 3),
+                ("position_stride", ctypes.c_int64 * 2)]
+
+
+class NormParams(ctypes.Structure):  # struct mvr_norm_params
+    _fields_ = [("rows", ctypes.c_int64), ("dim", ctypes.c_int32), ("residual_type", ctypes.c_int32), ("branch_type", ctypes.c_int32),
+                ("param_type", ctypes.c_int32), ("kind", ctypes.c_int32), ("reserved_", ctypes.c_int32), ("gate_groups", ctypes.c_int64),
+                ("scale_groups", ctypes.c_int64), ("scale", ctypes.c_float), ("eps", ctypes.c_float)]
+
+
 # name -> (restype, argtypes); mirrors include/mvr.h one to one
 _MB, _MP, _PP = ctypes.POINTER(MeshBatch), ctypes.POINTER(MeshParams), ctypes.POINTER(PointsParams)
 _PL = ctypes.POINTER(PackLayout)
+_RP, _NP = ctypes.POINTER(RotaryParams), ctypes.POINTER(NormParams)
 PROTOTYPES = {
+    "mvr_rotate_tokens_forward": (ctypes.c_int, [_RP] + [_vp] * 5),
+    "mvr_rotate_tokens_backward": (ctypes.c_int, [_RP] + [_vp] * 7),
+    "mvr_add_norm_tokens_forward": (ctypes.c_int, [_NP] + [_vp] * 11),
+    "mvr_add_norm_tokens_workspace_bytes": (ctypes.c_size_t, [_NP]),
+    "mvr_add_norm_tokens_backward": (ctypes.c_int, [_NP] + [_vp] * 16 + [ctypes.c_size_t, _vp]),
     "mvr_regularize_views_forward": (ctypes.c_int, [_vp] + [ctypes.c_int32] * 4 + [_vp] * 4 + [ctypes.c_int32, _vp, _vp]),
     "mvr_regularize_views_backward": (ctypes.c_int, [_vp] + [ctypes.c_int32] * 4 + [_vp] * 4 + [ctypes.c_int32, _vp, _vp]),
     "mvr_regularize_normalize_views_forward": (ctypes.c_int, [_vp] + [ctypes.c_int32] * 4 + [_vp] * 4 + [ctypes.c_int32, c_float_p, c_float_p, _vp, _vp]),

@@ -7,6 +7,7 @@ import hashlib
 import os
 import shutil
 import subprocess
+from concurrent.futures import ThreadPoolExecutor
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_HERE, "csrc")
@@ -22,6 +23,10 @@ HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
                # the hand-written two-pixel arithmetic (explicit float2 types) is not affected
                "-fno-slp-vectorize"]
 
+# the kernels on view tokens: contraction to fused multiply-adds is wanted there, packed f32 arithmetic is kept out
+TOKEN_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=fast", "-fno-fast-math", "-fno-slp-vectorize",
+               "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
 
 def _stale(target, sources):
     if not os.path.exists(target):
@@ -36,7 +41,12 @@ def _sources():
     # the rest only take part in the staleness check
     import glob
     return [os.path.join(CSRC, "mvr_kernels.hip"), os.path.join(CSRC, "mvr_math.h"), inc, os.path.join(CSRC, "mvr_pack.cpp"),
-            os.path.join(CSRC, "mvr_regularize.hip")] + sorted(glob.glob(os.path.join(CSRC, "*.inc")))
+            os.path.join(CSRC, "mvr_regularize.hip")] + sorted(glob.glob(os.path.join(CSRC, "*.inc"))) + _token_sources() + [
+                os.path.join(CSRC, "mvr_token_types.h")]
+
+
+def _token_sources():
+    return [os.path.join(CSRC, "mvr_tokens.hip")]
 
 
 def _src_hash(srcs, flags):
@@ -56,7 +66,7 @@ def _hash_path(lib):
 
 def source_hash():
     """The hash the product library carries (mvr_source_hash()) when it was built from the sources on disk."""
-    return _src_hash(_sources(), HIPCC_FLAGS)
+    return _src_hash(_sources(), HIPCC_FLAGS + TOKEN_FLAGS)
 
 
 def is_current(lib=None):
@@ -91,7 +101,7 @@ def build_hip(force=False, verbose=False, out=None, extra_flags=()):
             _compile(srcs, LIB_PATH, [], verbose)
             tmp = "%s.tmp.%d" % (_hash_path(LIB_PATH), os.getpid())
             with open(tmp, "w") as f:
-                f.write(_src_hash(srcs, HIPCC_FLAGS) + "\n")
+                f.write(source_hash() + "\n")
             os.replace(tmp, _hash_path(LIB_PATH))
         finally:
             fcntl.flock(lock, fcntl.LOCK_UN)
@@ -105,19 +115,27 @@ def _compile(srcs, LIB_PATH, extra, verbose):
     # finished library is renamed into place (atomic on POSIX).
     tmp_lib = "%s.tmp.%d" % (LIB_PATH, os.getpid())
     pack_o = "%s.pack.%d.o" % (LIB_PATH, os.getpid())
-    cmds = [["g++", "-O3", "-std=c++17", "-fPIC", "-fvisibility-inlines-hidden", "-c", "-o", pack_o, srcs[3]],
-            [hipcc] + HIPCC_FLAGS + extra + ['-DMVR_SRC_HASH="%s"' % _src_hash(srcs, HIPCC_FLAGS), "-o", tmp_lib, srcs[0], srcs[4],
-                                               "-Wl," + pack_o]]
+    # the kernels on view tokens have flags of their own and are compiled beside the rest
+    objs = {src: "%s.%s.%d.o" % (LIB_PATH, os.path.splitext(os.path.basename(src))[0], os.getpid()) for src in [srcs[0], srcs[4]] + _token_sources()}
+    hash_flag = ['-DMVR_SRC_HASH="%s"' % source_hash()]
+    flags = {src: TOKEN_FLAGS if src in _token_sources() else [f for f in HIPCC_FLAGS if f != "-shared"] + hash_flag for src in objs}
+    cmds = [["g++", "-O3", "-std=c++17", "-fPIC", "-fvisibility-inlines-hidden", "-c", "-o", pack_o, srcs[3]]] + [
+        [hipcc] + flags[src] + extra + ["-c", "-o", o, src] for src, o in objs.items()]
+    link = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", tmp_lib] + list(objs.values()) + [pack_o]
+
+    def run(cmd):
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError("%s failed:\n%s\n%s" % (os.path.basename(cmd[0]), " ".join(cmd), r.stderr))
+        if verbose:
+            print(" ".join(cmd))
     try:
-        for cmd in cmds:
-            r = subprocess.run(cmd, capture_output=True, text=True)
-            if r.returncode != 0:
-                raise RuntimeError("%s failed:\n%s\n%s" % (os.path.basename(cmd[0]), " ".join(cmd), r.stderr))
-            if verbose:
-                print(" ".join(cmd))
+        with ThreadPoolExecutor(len(cmds)) as pool:
+            list(pool.map(run, cmds))
+        run(link)
         os.replace(tmp_lib, LIB_PATH)
     finally:
-        for f in (pack_o, tmp_lib):
+        for f in [pack_o, tmp_lib] + list(objs.values()):
             if os.path.exists(f):
                 os.remove(f)
     return LIB_PATH

@@ -1,0 +1,614 @@
+// The tokens of rendered views, where a network takes them up after the renderer and the regulariser: rotary positions with several axes, and the
+// norms around a block with its gate and residual scale.  (Attention over the tokens: mvr_attend.hip.)
+//
+// Both operators are bound by HBM: every kernel here reads each input once and writes each output once, all arithmetic in 32 bits
+// (angles in 64), one rounding at the store.
+#include <math.h>
+
+#include "mvr_token_types.h"
+
+using namespace mvr_tok;
+
+namespace {
+
+// ======================================================================================
+// rotary positions
+// ======================================================================================
+//
+// Pair i of a head turns by th_i = 2 pi pos[axis(i)] turns_i:  y1 = x1 cos - x2 sin,  y2 = x1 sin + x2 cos.
+// The product pos * turns is formed and reduced to a fraction of a turn in 64 bits: at position 1e5 a 32-bit product is off by 4e-3 turns.
+// Backward: dx is dy turned back, and dL/dth_i = x1 dx2 - x2 dx1 (a rotation leaves that determinant alone, so x and dx serve as
+// well as y and dy), summed over the heads and, times 2 pi turns_i, over the pairs of an axis — in a fixed order, without atomics.
+//
+// A workgroup takes `tb` tokens: their cosines and sines go to LDS once (one 64-bit reduction and one sincospi per pair, shared by the
+// heads), then thread (token, unit of 16 bytes, head slice) keeps the cosines of its pairs in registers and walks its heads: one
+// 16-byte load and store per half of a pair, nothing else in the loop.
+
+constexpr int kBlock = 256;
+constexpr int kMaxPairs = 128;
+
+struct RotArgs {
+  const void *x, *g;      // x (forward; backward only where the positions' gradient is asked for), grad_out
+  void *out;              // out / grad_x, contiguous
+  const float *pos;
+  float *gpos;            // (B, L, axes) or null
+  int64_t xs[3], gs[3], ps[2];
+  int64_t rows;           // B * L
+  int32_t L, H, D, n;     // n: pairs
+  int32_t units, rest;    // 16-byte units of rotated pairs / all units of a head
+  int32_t tb, hs;         // tokens and head slices of a workgroup
+  int32_t axes, end[4];   // end[a]: first pair behind axis a
+  double turns[kMaxPairs];
+};
+
+template <typename T, bool INTER, bool BWD, bool GPOS>
+__global__ __launch_bounds__(kBlock) void k_rotate_tokens(RotArgs a) {
+  constexpr int VE = 16 / sizeof(T);            // elements of a unit's vector
+  constexpr int NP = INTER ? VE / 2 : VE;       // pairs of a unit
+  extern __shared__ float2 cs[];                // [tb][n]; then, with GPOS, the slopes [hs][tb][n] as floats
+  const int tid = threadIdx.x;
+  const int64_t row0 = (int64_t)blockIdx.x * a.tb;
+  const int here = (int)(a.rows - row0 < a.tb ? a.rows - row0 : a.tb);
+  for (int e = tid; e < here * a.n; e += kBlock) {
+    const int t = e / a.n, i = e - t * a.n;
+    int axis = 0;
+    for (int k = 0; k + 1 < a.axes; ++k) axis += i >= a.end[k];
+    const int64_t row = row0 + t, b = row / a.L, l = row - b * a.L;
+    const double p = (double)a.pos[b * a.ps[0] + l * a.ps[1] + axis] * a.turns[i];
+    const float r = (float)(p - rint(p));
+    float s, c;
+    sincospif(2.0f * r, &s, &c);
+    cs[e] = make_float2(c, BWD ? -s : s);
+  }
+  __syncthreads();
+  float *slopes = reinterpret_cast<float *>(cs + a.tb * a.n);
+  const int u = tid % a.rest, q = tid / a.rest, t = q % a.tb, slice = q / a.tb;
+  if (slice < a.hs && t < here) {
+    const int64_t row = row0 + t, b = row / a.L, l = row - b * a.L;
+    const T *in = (const T *)(BWD ? a.g : a.x) + (BWD ? b * a.gs[0] + l * a.gs[1] : b * a.xs[0] + l * a.xs[1]);
+    const int64_t in_h = BWD ? a.gs[2] : a.xs[2];
+    const T *x = (const T *)a.x + (GPOS ? b * a.xs[0] + l * a.xs[1] : 0);
+    T *out = (T *)a.out + row * a.H * a.D;
+    if (u < a.units) {
+      const int i0 = u * NP;                    // first pair
+      float c[NP], s[NP], th[NP];
+#pragma unroll
+      for (int k = 0; k < NP; ++k) {
+        const bool on = i0 + k < a.n;
+        const float2 v = on ? cs[t * a.n + i0 + k] : make_float2(1.0f, 0.0f);
+        c[k] = v.x, s[k] = v.y, th[k] = 0.0f;
+      }
+      // where the unit's vectors lie in a head, and how much of them is there
+      const int at1 = INTER ? 2 * i0 : i0, at2 = a.n + i0;
+      const int left = INTER ? a.D - at1 : a.n - i0;
+      const int live = a.n - i0;                // pairs behind it (interleaved: the head's tail in this vector) stay as they are
+#pragma unroll 4
+      for (int h = slice; h < a.H; h += a.hs) {
+        const T *p = in + h * in_h;
+        T *o = out + (int64_t)h * a.D;
+        float v[VE], w[VE], xv[VE], xw[VE];
+        load_n<VE>(p + at1, left, v);
+        if constexpr (!INTER) load_n<VE>(p + at2, left, w);
+        if constexpr (GPOS) {
+          load_n<VE>(x + h * a.xs[2] + at1, left, xv);
+          if constexpr (!INTER) load_n<VE>(x + h * a.xs[2] + at2, left, xw);
+        }
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+          const float e1 = INTER ? v[2 * k] : v[k], e2 = INTER ? v[2 * k + 1] : w[k];
+          const float r1 = e1 * c[k] - e2 * s[k], r2 = e1 * s[k] + e2 * c[k];
+          if constexpr (GPOS) {
+            const float x1 = INTER ? xv[2 * k] : xv[k], x2 = INTER ? xv[2 * k + 1] : xw[k];
+            th[k] += k < live ? x1 * r2 - x2 * r1 : 0.0f;
+          }
+          if constexpr (INTER) {
+            v[2 * k] = k < live ? r1 : e1;
+            v[2 * k + 1] = k < live ? r2 : e2;
+          } else {
+            v[k] = r1, w[k] = r2;
+          }
+        }
+        store_n<VE>(o + at1, left, v);
+        if constexpr (!INTER) store_n<VE>(o + at2, left, w);
+      }
+      if constexpr (GPOS) {
+#pragma unroll
+        for (int k = 0; k < NP; ++k)
+          if (k < live) slopes[(slice * a.tb + t) * a.n + i0 + k] = th[k];
+      }
+    } else {                                    // the head's part behind the pairs
+      const int at = (INTER ? a.units * VE : 2 * a.n) + (u - a.units) * VE;
+      for (int h = slice; h < a.H; h += a.hs) {
+        float v[VE];
+        load_n<VE>(in + h * in_h + at, a.D - at, v);
+        store_n<VE>(out + (int64_t)h * a.D + at, a.D - at, v);
+      }
+    }
+  }
+  if constexpr (GPOS) {
+    __syncthreads();
+    for (int e = tid; e < here * a.axes; e += kBlock) {
+      const int t1 = e / a.axes, ax = e - t1 * a.axes;
+      float sum = 0.0f;
+      for (int i = ax ? a.end[ax - 1] : 0; i < a.end[ax]; ++i) {
+        float th = 0.0f;
+        for (int k = 0; k < a.hs; ++k) th += slopes[(k * a.tb + t1) * a.n + i];
+        sum += th * (float)(2.0 * M_PI * a.turns[i]);
+      }
+      a.gpos[(row0 + t1) * a.axes + ax] = sum;
+    }
+  }
+}
+
+int type_size(int t) { return t == MVR_TYPE_FLOAT ? 4 : t == MVR_TYPE_HALF || t == MVR_TYPE_BFLOAT ? 2 : 0; }
+
+int rotary_args(RotArgs &a, const mvr_rotary_params *p, const double *turns) {
+  if (!p || !turns) return bad("mvr_rotate_tokens: params and turns must be given");
+  if (p->batch <= 0 || p->tokens <= 0 || p->heads <= 0 || p->dim <= 0 || p->dim > 256 || p->heads > (1 << 20))
+    return bad("mvr_rotate_tokens: bad shape (batch, tokens, heads >= 1, 1 <= dim <= 256)");
+  if (!type_size(p->type)) return bad("mvr_rotate_tokens: unknown type");
+  if (p->reserved_) return bad("mvr_rotate_tokens: reserved_ must be 0");
+  if (p->axes < 1 || p->axes > 4) return bad("mvr_rotate_tokens: 1 to 4 axes");
+  int n = 0;
+  for (int k = 0; k < p->axes; ++k) {
+    if (p->sections[k] < 1 || p->sections[k] > kMaxPairs) return bad("mvr_rotate_tokens: a section needs at least one pair");
+    n += p->sections[k];
+    a.end[k] = n;
+  }
+  if (2 * n > p->dim) return bad("mvr_rotate_tokens: the sections' pairs do not fit the head dimension");
+  if (p->interleaved && p->dim % 2) return bad("mvr_rotate_tokens: interleaved pairs need an even head dimension");
+  const int ve = 16 / type_size(p->type), np = p->interleaved ? ve / 2 : ve;
+  a.rows = (int64_t)p->batch * p->tokens;
+  a.L = p->tokens, a.H = p->heads, a.D = p->dim, a.n = n, a.axes = p->axes;
+  for (int k = 0; k < 3; ++k) a.xs[k] = p->x_stride[k], a.gs[k] = p->grad_stride[k];
+  a.ps[0] = p->position_stride[0], a.ps[1] = p->position_stride[1];
+  if (p->interleaved) {
+    a.units = (n + np - 1) / np;
+    const int in_units = a.units * ve;   // the last unit's vector also holds the tail that fits behind its pairs
+    a.rest = a.units + (p->dim > in_units ? (p->dim - in_units + ve - 1) / ve : 0);
+  } else {
+    a.units = (n + np - 1) / np;
+    a.rest = a.units + (p->dim - 2 * n + ve - 1) / ve;
+  }
+  // head slices: up to four threads share a (token, unit), so that a token's angles serve many heads and the workgroup still holds
+  // several tokens
+  a.hs = p->heads < 4 ? p->heads : 4;
+  while (a.hs > 1 && a.rest * a.hs > kBlock) --a.hs;
+  a.tb = kBlock / (a.rest * a.hs);
+  if (a.tb > a.rows) a.tb = (int)a.rows;
+  if (a.tb < 1) a.tb = 1;
+  for (int k = 0; k < n; ++k) a.turns[k] = turns[k];
+  return MVR_OK;
+}
+
+template <typename T>
+int launch_rotary_t(const RotArgs &a, bool inter, bool bwd, hipStream_t st) {
+  const int64_t blocks = (a.rows + a.tb - 1) / a.tb;
+  if (blocks > 0x7FFFFFFF) return bad("mvr_rotate_tokens: too many tokens");
+  const size_t lds = (size_t)a.tb * a.n * (sizeof(float2) + (a.gpos ? a.hs * sizeof(float) : 0));
+  const dim3 g((unsigned)blocks), b(kBlock);
+  if (!bwd) {
+    if (inter) hipLaunchKernelGGL((k_rotate_tokens<T, true, false, false>), g, b, lds, st, a);
+    else hipLaunchKernelGGL((k_rotate_tokens<T, false, false, false>), g, b, lds, st, a);
+  } else if (!a.gpos) {
+    if (inter) hipLaunchKernelGGL((k_rotate_tokens<T, true, true, false>), g, b, lds, st, a);
+    else hipLaunchKernelGGL((k_rotate_tokens<T, false, true, false>), g, b, lds, st, a);
+  } else {
+    if (inter) hipLaunchKernelGGL((k_rotate_tokens<T, true, true, true>), g, b, lds, st, a);
+    else hipLaunchKernelGGL((k_rotate_tokens<T, false, true, true>), g, b, lds, st, a);
+  }
+  return launched("k_rotate_tokens");
+}
+
+int launch_rotary(const RotArgs &a, int type, bool inter, bool bwd, mvr_stream_t stream) {
+  const hipStream_t st = (hipStream_t)stream;
+  return type == MVR_TYPE_FLOAT ? launch_rotary_t<float>(a, inter, bwd, st)
+         : type == MVR_TYPE_HALF ? launch_rotary_t<f16>(a, inter, bwd, st) : launch_rotary_t<bf16>(a, inter, bwd, st);
+}
+
+// ======================================================================================
+// norms around a block
+// ======================================================================================
+//
+//   n = post N(branch)  (or branch),   y = residual + s g n,   z = N(y) weight + bias
+// N divides a row by the root of its mean square (+ eps), after taking its mean off for kind "layer".  A row lives in the registers of one
+// wave (up to 2048 wide forward, 1024 backward) or of a workgroup: one read, both norms' statistics by wave sums, one write.
+//
+// Backward, with r = 1 / std and hats for normed rows:
+//   dyt = dy + r_y (dz w - <dz w> - yhat <dz w yhat>)        (<>: mean over the row; the first mean only for "layer")
+//   dresidual = dyt,  dn = s g dyt,  dbranch = r_a (dn post - <dn post> - ahat <dn post ahat>)
+// and the column sums dweight = sum dz yhat, dbias = sum dz, dpost = sum dn ahat, dgate = sum s post ahat dyt.  A workgroup sums the columns
+// of its rows in registers and leaves one line of partial sums; k_norm_columns adds the lines up in a fixed order.
+
+struct NormArgs {
+  const void *residual, *branch, *weight, *bias, *post, *gate;
+  const float *scale;
+  void *y, *z;
+  float *stats;             // (rows, 4): mean and 1 / std of y, of branch
+  // backward: residual = y as stored, dy / dz either may be null
+  const void *dy, *dz;
+  void *dresidual, *dbranch;
+  float *partial;           // (blocks, 4, D): dweight, dbias, dpost, dgate
+  int64_t rows, group_rows, scale_rows, block_rows;
+  int32_t D, layer, ptype, blocks_per_group;
+  float s, eps;
+};
+
+__device__ __forceinline__ void load_param(const void *p, int type, int64_t at, int left, float (&v)[8]) {
+  if (type == MVR_TYPE_FLOAT) load_n<8>((const float *)p + at, left, v);
+  else if (type == MVR_TYPE_HALF) load_n<8>((const f16 *)p + at, left, v);
+  else load_n<8>((const bf16 *)p + at, left, v);
+}
+
+// sums over the row of K values at once; with WAVES > 1 through LDS, in wave order (two buffers: one barrier a call)
+template <int WAVES, int K>
+__device__ __forceinline__ void row_sum(float (&v)[K], float *lds, int &turn) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = wave_sum(v[k]);
+  if constexpr (WAVES > 1) {
+    float *at = lds + turn * WAVES * 2;
+    turn ^= 1;
+    const int wave = threadIdx.x / 64;
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) at[wave * 2 + k] = v[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      v[k] = 0.0f;
+      for (int w = 0; w < WAVES; ++w) v[k] += at[w * 2 + k];
+    }
+  }
+}
+
+// mean (0 for rms) and 1 / std of a row held as v; places behind the row hold zeros and are left out of the second sum
+template <int WAVES, int NV>
+__device__ __forceinline__ float2 row_stats(const float (&v)[NV][8], const int (&left)[NV], const NormArgs &a, float *lds, int &turn) {
+  float m = 0.0f;
+  const float inv = 1.0f / (float)a.D;
+  if (a.layer) {
+    float s[1] = {0.0f};
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s[0] += v[j][k];
+    row_sum<WAVES>(s, lds, turn);
+    m = s[0] * inv;
+  }
+  float q[1] = {0.0f};
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float d = k < left[j] ? v[j][k] - m : 0.0f;
+      q[0] += d * d;
+    }
+  row_sum<WAVES>(q, lds, turn);
+  return make_float2(m, 1.0f / sqrtf(q[0] * inv + a.eps));
+}
+
+template <typename TR, typename TB, int WAVES, int NV>
+__global__ __launch_bounds__(kBlock) void k_add_norm(NormArgs a) {
+  __shared__ float lds[16];
+  int turn = 0;
+  const int lane = WAVES > 1 ? threadIdx.x : threadIdx.x & 63;
+  constexpr int kRows = WAVES > 1 ? 1 : kBlock / 64, kLanes = 64 * WAVES;
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  int left[NV];
+  float w[NV][8], bi[NV][8], po[NV][8];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = (lane + j * kLanes) * 8;
+    left[j] = a.D - c < 0 ? 0 : a.D - c;
+    load_param(a.weight, a.ptype, c, left[j], w[j]);
+    if (a.bias) load_param(a.bias, a.ptype, c, left[j], bi[j]);
+    if (a.post) load_param(a.post, a.ptype, c, left[j], po[j]);
+  }
+  for (int64_t row = (int64_t)blockIdx.x * kRows + (WAVES > 1 ? 0 : threadIdx.x / 64); row < a.rows; row += step) {
+    const TR *rp = (const TR *)a.residual + row * a.D;
+    const TB *bp = (const TB *)a.branch + row * a.D;
+    float v[NV][8], n[NV][8];
+    const float s = a.scale ? a.scale[row / a.scale_rows] : a.s;
+    const bool dropped = a.scale && s == 0.0f;   // a dropped view's branch is not read: whatever it holds stays out
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      load_n<8>(rp + (lane + j * kLanes) * 8, left[j], v[j]);
+      load_n<8>(bp + (lane + j * kLanes) * 8, dropped ? 0 : left[j], n[j]);
+    }
+    float2 sa = make_float2(0.0f, 1.0f);
+    if (a.post) sa = row_stats<WAVES, NV>(n, left, a, lds, turn);
+    if (!dropped) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        float g[8];
+        if (a.gate) load_param(a.gate, a.ptype, (row / a.group_rows) * a.D + (lane + j * kLanes) * 8, left[j], g);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          float t = a.post ? (n[j][k] - sa.x) * sa.y * po[j][k] : n[j][k];
+          if (a.gate) t *= g[k];
+          if (k < left[j]) v[j][k] += s * t;
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) store_n<8>((TR *)a.y + row * a.D + (lane + j * kLanes) * 8, left[j], v[j]);
+    const float2 sy = row_stats<WAVES, NV>(v, left, a, lds, turn);
+    if (a.stats && lane == 0) *reinterpret_cast<float4 *>(a.stats + row * 4) = make_float4(sy.x, sy.y, sa.x, sa.y);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        v[j][k] = (v[j][k] - sy.x) * sy.y * w[j][k];
+        if (a.bias) v[j][k] += bi[j][k];
+      }
+      store_n<8>((TB *)a.z + row * a.D + (lane + j * kLanes) * 8, left[j], v[j]);
+    }
+  }
+}
+
+template <typename TR, typename TB, int WAVES, int NV>
+__global__ __launch_bounds__(kBlock) void k_add_norm_backward(NormArgs a) {
+  constexpr int kRows = WAVES > 1 ? 1 : kBlock / 64, kLanes = 64 * WAVES;
+  __shared__ float lds[16];
+  __shared__ float cols[WAVES > 1 ? 1 : kRows][WAVES > 1 ? 1 : kLanes * 8];
+  int turn = 0;
+  const int lane = WAVES > 1 ? threadIdx.x : threadIdx.x & 63, wave = WAVES > 1 ? 0 : threadIdx.x / 64;
+  const int64_t group = blockIdx.x / a.blocks_per_group, part = blockIdx.x - group * a.blocks_per_group;
+  const int64_t first = group * a.group_rows + part * a.block_rows;
+  const int64_t end_g = (group + 1) * a.group_rows, last = first + a.block_rows < end_g ? first + a.block_rows : end_g;
+  const float inv = 1.0f / (float)a.D;
+  int left[NV];
+  float w[NV][8], po[NV][8], ga[NV][8];
+  float dw[NV][8], db[NV][8], dp[NV][8], dg[NV][8];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = (lane + j * kLanes) * 8;
+    left[j] = a.D - c < 0 ? 0 : a.D - c;
+    load_param(a.weight, a.ptype, c, left[j], w[j]);
+    if (a.post) load_param(a.post, a.ptype, c, left[j], po[j]);
+    if (a.gate) load_param(a.gate, a.ptype, group * a.D + c, left[j], ga[j]);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (!a.post) po[j][k] = 1.0f;
+      if (!a.gate) ga[j][k] = 1.0f;
+      dw[j][k] = db[j][k] = dp[j][k] = dg[j][k] = 0.0f;
+    }
+  }
+  for (int64_t row = first + wave; row < last; row += kRows) {
+    const float s = a.scale ? a.scale[row / a.scale_rows] : a.s;
+    const bool dropped = a.scale && s == 0.0f;
+    const float4 st = *reinterpret_cast<const float4 *>(a.stats + row * 4);
+    float y[NV][8], n[NV][8], g[NV][8], t[NV][8];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int64_t at = row * a.D + (lane + j * kLanes) * 8;
+      load_n<8>((const TR *)a.residual + at, left[j], y[j]);
+      load_n<8>((const TB *)a.branch + at, dropped ? 0 : left[j], n[j]);
+      load_n<8>((const TB *)a.dz + at, a.dz ? left[j] : 0, g[j]);
+      load_n<8>((const TR *)a.dy + at, a.dy ? left[j] : 0, t[j]);
+    }
+    float m[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        y[j][k] = k < left[j] ? (y[j][k] - st.x) * st.y : 0.0f;   // yhat
+        dw[j][k] += g[j][k] * y[j][k];
+        db[j][k] += g[j][k];
+        g[j][k] *= w[j][k];
+        m[0] += g[j][k] * y[j][k];
+        m[1] += g[j][k];
+      }
+    row_sum<WAVES>(m, lds, turn);
+    const float m0 = m[0] * inv, m1 = a.layer ? m[1] * inv : 0.0f;
+    float d[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        t[j][k] += st.y * (g[j][k] - m1 - y[j][k] * m0);          // dyt
+        const float hat = dropped || k >= left[j] ? 0.0f : a.post ? (n[j][k] - st.z) * st.w : n[j][k];
+        const float u = k < left[j] ? s * t[j][k] : 0.0f;
+        dg[j][k] += u * po[j][k] * hat;
+        const float dn = dropped ? 0.0f : u * ga[j][k];
+        dp[j][k] += dn * hat;
+        n[j][k] = hat;
+        g[j][k] = dn * po[j][k];
+        d[0] += g[j][k] * hat;
+        d[1] += g[j][k];
+      }
+      store_n<8>((TR *)a.dresidual + row * a.D + (lane + j * kLanes) * 8, left[j], t[j]);
+    }
+    if (a.post) {
+      row_sum<WAVES>(d, lds, turn);
+      const float d0 = d[0] * inv, d1 = a.layer ? d[1] * inv : 0.0f;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) g[j][k] = dropped ? 0.0f : st.w * (g[j][k] - d1 - n[j][k] * d0);
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) store_n<8>((TB *)a.dbranch + row * a.D + (lane + j * kLanes) * 8, left[j], g[j]);
+  }
+  if (!a.partial) return;
+  float *line = a.partial + (int64_t)blockIdx.x * 4 * a.D;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = q == 0 ? dw[j][k] : q == 1 ? db[j][k] : q == 2 ? dp[j][k] : dg[j][k];
+      if constexpr (WAVES > 1) {
+        store_n<8>(line + q * a.D + (lane + j * kLanes) * 8, left[j], v);
+      } else {   // the four waves' rows, in wave order
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) cols[wave][lane + k * 64] = v[k];
+        __syncthreads();
+        for (int e = threadIdx.x; e < 512; e += kBlock) {
+          const int l = e >> 3, k = e & 7, c = (l + j * kLanes) * 8 + k;
+          if (c < a.D) line[q * a.D + c] = (cols[0][l + k * 64] + cols[1][l + k * 64]) + (cols[2][l + k * 64] + cols[3][l + k * 64]);
+        }
+      }
+    }
+  }
+}
+
+// 64 columns of one of the four sums: sixteen waves add the lines k, k + 16, ..., then wave 0 adds the waves' sums up
+__global__ __launch_bounds__(1024) void k_norm_columns(const float *partial, int32_t D, int32_t blocks, int32_t blocks_per_group, int32_t ptype,
+                                                       void *dweight, void *dbias, void *dpost, void *dgate) {
+  __shared__ float lds[16][64];
+  const int q = blockIdx.y < 3 ? blockIdx.y : 3;
+  const int64_t group = blockIdx.y < 3 ? 0 : blockIdx.y - 3;
+  void *out = q == 0 ? dweight : q == 1 ? dbias : q == 2 ? dpost : dgate;
+  if (!out) return;
+  const int first = q == 3 ? (int)group * blocks_per_group : 0, last = q == 3 ? first + blocks_per_group : blocks;
+  const int wave = threadIdx.x / 64, lane = threadIdx.x & 63, c = blockIdx.x * 64 + lane;
+  float s = 0.0f;
+  if (c < D)
+    for (int k = first + wave; k < last; k += 16) s += partial[((int64_t)k * 4 + q) * D + c];
+  lds[wave][lane] = s;
+  __syncthreads();
+  if (wave == 0 && c < D) {
+    s = 0.0f;
+    for (int k = 0; k < 16; ++k) s += lds[k][lane];
+    const int64_t at = group * D + c;
+    if (ptype == MVR_TYPE_FLOAT) ((float *)out)[at] = s;
+    else if (ptype == MVR_TYPE_HALF) ((f16 *)out)[at] = (f16)s;
+    else ((bf16 *)out)[at] = (bf16)s;
+  }
+}
+
+int norm_args(NormArgs &a, const mvr_norm_params *p) {
+  if (!p) return bad("mvr_add_norm_tokens: params must be given");
+  if (p->rows <= 0 || p->dim <= 0 || p->dim > 8192) return bad("mvr_add_norm_tokens: rows >= 1 and 1 <= dim <= 8192");
+  const int r = p->residual_type, b = p->branch_type;
+  if (!type_size(r) || !type_size(b) || !type_size(p->param_type)) return bad("mvr_add_norm_tokens: unknown type");
+  if (r != b && r != MVR_TYPE_FLOAT) return fail(MVR_ERR_UNSUPPORTED, "mvr_add_norm_tokens: the residual has the branch's type or 32 bits");
+  if (p->reserved_) return bad("mvr_add_norm_tokens: reserved_ must be 0");
+  if (p->kind != 0 && p->kind != 1) return bad("mvr_add_norm_tokens: kind is 0 (rms) or 1 (layer)");
+  if (p->gate_groups < 0 || p->scale_groups < 0 || (p->gate_groups && p->rows % p->gate_groups) || (p->scale_groups && p->rows % p->scale_groups))
+    return bad("mvr_add_norm_tokens: the groups of gate and scale must divide the rows");
+  if (!(p->eps >= 0.0f)) return bad("mvr_add_norm_tokens: eps must not be negative");
+  a.rows = p->rows, a.D = p->dim, a.layer = p->kind, a.ptype = p->param_type, a.s = p->scale, a.eps = p->eps;
+  a.group_rows = p->gate_groups ? p->rows / p->gate_groups : p->rows;
+  a.scale_rows = p->scale_groups ? p->rows / p->scale_groups : p->rows;
+  return MVR_OK;
+}
+
+// Workgroups of the backward: about 1024 in all, each with a run of rows of one gate group
+void norm_blocks(const mvr_norm_params *p, int64_t &per_group, int64_t &rows_each, int64_t &blocks) {
+  const int64_t groups = p->gate_groups ? p->gate_groups : 1, rows = p->rows / groups;
+  const int64_t least = p->dim > 1024 ? 2 : 8;   // rows of a workgroup: below, the partial sums would weigh more than the rows
+  per_group = (1024 + groups - 1) / groups;
+  if (per_group > (rows + least - 1) / least) per_group = (rows + least - 1) / least;
+  rows_each = (rows + per_group - 1) / per_group;
+  per_group = (rows + rows_each - 1) / rows_each;
+  blocks = per_group * groups;
+}
+
+template <typename TR, typename TB>
+int launch_norm(const NormArgs &a, hipStream_t st) {
+  const bool wide = a.D > 2048;
+  int64_t blocks = wide ? a.rows : (a.rows + 3) / 4;
+  if (blocks > 2048) blocks = 2048;
+  const dim3 g((unsigned)blocks), b(kBlock);
+  if (a.D <= 512) hipLaunchKernelGGL((k_add_norm<TR, TB, 1, 1>), g, b, 0, st, a);
+  else if (a.D <= 1024) hipLaunchKernelGGL((k_add_norm<TR, TB, 1, 2>), g, b, 0, st, a);
+  else if (a.D <= 2048) hipLaunchKernelGGL((k_add_norm<TR, TB, 1, 4>), g, b, 0, st, a);
+  else if (a.D <= 4096) hipLaunchKernelGGL((k_add_norm<TR, TB, 4, 2>), g, b, 0, st, a);
+  else hipLaunchKernelGGL((k_add_norm<TR, TB, 4, 4>), g, b, 0, st, a);
+  return launched("k_add_norm");
+}
+
+template <typename TR, typename TB>
+int launch_norm_backward(const NormArgs &a, int64_t blocks, hipStream_t st) {
+  const dim3 g((unsigned)blocks), b(kBlock);
+  if (a.D <= 512) hipLaunchKernelGGL((k_add_norm_backward<TR, TB, 1, 1>), g, b, 0, st, a);
+  else if (a.D <= 1024) hipLaunchKernelGGL((k_add_norm_backward<TR, TB, 1, 2>), g, b, 0, st, a);
+  else if (a.D <= 2048) hipLaunchKernelGGL((k_add_norm_backward<TR, TB, 4, 1>), g, b, 0, st, a);
+  else if (a.D <= 4096) hipLaunchKernelGGL((k_add_norm_backward<TR, TB, 4, 2>), g, b, 0, st, a);
+  else hipLaunchKernelGGL((k_add_norm_backward<TR, TB, 4, 4>), g, b, 0, st, a);
+  return launched("k_add_norm_backward");
+}
+
+#define MVR_NORM_TYPES(fn, p, ...)                                                                                                        \
+  ((p)->residual_type == MVR_TYPE_FLOAT                                                                                                   \
+       ? ((p)->branch_type == MVR_TYPE_FLOAT ? fn<float, float>(__VA_ARGS__)                                                              \
+                                             : (p)->branch_type == MVR_TYPE_HALF ? fn<float, f16>(__VA_ARGS__) : fn<float, bf16>(__VA_ARGS__)) \
+       : (p)->residual_type == MVR_TYPE_HALF ? fn<f16, f16>(__VA_ARGS__) : fn<bf16, bf16>(__VA_ARGS__))
+
+}  // namespace
+
+extern "C" int mvr_rotate_tokens_forward(const mvr_rotary_params *params, const double *turns, const void *x, const float *positions, void *out,
+                                         mvr_stream_t stream) {
+  RotArgs a = {};
+  if (!x || !positions || !out || x == out) return bad("mvr_rotate_tokens_forward: x, positions and out must be given, x and out distinct");
+  if (int rc = rotary_args(a, params, turns)) return rc;
+  a.x = x, a.pos = positions, a.out = out;
+  return launch_rotary(a, params->type, params->interleaved != 0, false, stream);
+}
+
+extern "C" int mvr_rotate_tokens_backward(const mvr_rotary_params *params, const double *turns, const void *x, const float *positions,
+                                          const void *grad_out, void *grad_x, float *grad_positions, mvr_stream_t stream) {
+  RotArgs a = {};
+  if (!positions || !grad_out || !grad_x || grad_out == grad_x) return bad("mvr_rotate_tokens_backward: positions, grad_out and grad_x must be given, the last two distinct");
+  if ((x == nullptr) != (grad_positions == nullptr)) return bad("mvr_rotate_tokens_backward: x and grad_positions go together");
+  if (int rc = rotary_args(a, params, turns)) return rc;
+  a.x = x, a.g = grad_out, a.pos = positions, a.out = grad_x, a.gpos = grad_positions;
+  return launch_rotary(a, params->type, params->interleaved != 0, true, stream);
+}
+
+extern "C" size_t mvr_add_norm_tokens_workspace_bytes(const mvr_norm_params *params) {
+  NormArgs a = {};
+  if (norm_args(a, params) != MVR_OK) return 0;
+  int64_t per, each, blocks;
+  norm_blocks(params, per, each, blocks);
+  return (size_t)blocks * 4 * params->dim * sizeof(float);
+}
+
+extern "C" int mvr_add_norm_tokens_forward(const mvr_norm_params *params, const void *residual, const void *branch, const void *weight,
+                                           const void *bias, const void *post_weight, const void *gate, const float *scale, void *y, void *z,
+                                           float *stats, mvr_stream_t stream) {
+  NormArgs a = {};
+  if (int rc = norm_args(a, params)) return rc;
+  if (!residual || !branch || !weight || !y || !z) return bad("mvr_add_norm_tokens_forward: residual, branch, weight, y and z must be given");
+  if ((gate != nullptr) != (params->gate_groups > 0) || (scale != nullptr) != (params->scale_groups > 0))
+    return bad("mvr_add_norm_tokens_forward: gate and scale go with their groups");
+  if (z == y || z == residual || z == branch || y == branch) return bad("mvr_add_norm_tokens_forward: y and z must not overlap each other or the inputs");
+  a.residual = residual, a.branch = branch, a.weight = weight, a.bias = bias, a.post = post_weight, a.gate = gate, a.scale = scale;
+  a.y = y, a.z = z, a.stats = stats;
+  return MVR_NORM_TYPES(launch_norm, params, a, (hipStream_t)stream);
+}
+
+extern "C" int mvr_add_norm_tokens_backward(const mvr_norm_params *params, const void *y, const void *branch, const void *weight,
+                                            const void *post_weight, const void *gate, const float *scale, const float *stats, const void *grad_y,
+                                            const void *grad_z, void *grad_residual, void *grad_branch, void *grad_weight, void *grad_bias,
+                                            void *grad_post_weight, void *grad_gate, void *workspace, size_t workspace_bytes,
+                                            mvr_stream_t stream) {
+  NormArgs a = {};
+  if (int rc = norm_args(a, params)) return rc;
+  if (!y || !branch || !weight || !stats || (!grad_y && !grad_z) || !grad_residual || !grad_branch)
+    return bad("mvr_add_norm_tokens_backward: y, branch, weight, stats, one of grad_y and grad_z, grad_residual and grad_branch must be given");
+  if ((gate != nullptr) != (params->gate_groups > 0) || (scale != nullptr) != (params->scale_groups > 0))
+    return bad("mvr_add_norm_tokens_backward: gate and scale go with their groups");
+  if ((grad_gate && !gate) || (grad_post_weight && !post_weight)) return bad("mvr_add_norm_tokens_backward: a gradient of a parameter that is not there");
+  int64_t per, each, blocks;
+  norm_blocks(params, per, each, blocks);
+  if (blocks > 0x7FFFFFFF || params->gate_groups > 65000) return bad("mvr_add_norm_tokens_backward: too many gate groups");
+  const bool columns = grad_weight || grad_bias || grad_post_weight || grad_gate;
+  if (columns && (!workspace || workspace_bytes < (size_t)blocks * 4 * params->dim * sizeof(float)))
+    return fail(MVR_ERR_WORKSPACE, "mvr_add_norm_tokens_backward: the workspace is smaller than mvr_add_norm_tokens_workspace_bytes says");
+  a.residual = y, a.branch = branch, a.weight = weight, a.post = post_weight, a.gate = gate, a.scale = scale;
+  a.stats = const_cast<float *>(stats), a.dy = grad_y, a.dz = grad_z, a.dresidual = grad_residual, a.dbranch = grad_branch;
+  a.partial = columns ? (float *)workspace : nullptr;
+  a.blocks_per_group = (int32_t)per, a.block_rows = each;
+  if (int rc = MVR_NORM_TYPES(launch_norm_backward, params, a, blocks, (hipStream_t)stream)) return rc;
+  if (!columns) return MVR_OK;
+  const dim3 g((unsigned)((params->dim + 63) / 64), 3 + (grad_gate ? (unsigned)params->gate_groups : 0));
+  hipLaunchKernelGGL(k_norm_columns, g, dim3(1024), 0, (hipStream_t)stream, a.partial, params->dim, (int32_t)blocks, (int32_t)per,
+                     params->param_type, grad_weight, grad_bias, grad_post_weight, grad_gate);
+  return launched("k_norm_columns");
+}
