@@ -473,6 +473,30 @@ int mvr_add_norm_tokens_backward(const mvr_norm_params *params, const void *y, c
                                  void *grad_weight, void *grad_bias, void *grad_post_weight, void *grad_gate,
                                  void *workspace, size_t workspace_bytes, mvr_stream_t stream);
 
+/* Attention over tokens: out = softmax(scale q k^T over the kept keys) v, head by head; 16-bit tensors, heads of at most 128.
+ * heads is a multiple of kv_heads (consecutive heads share a key/value head).  keep: (batch, keep_groups) bytes, each for
+ * keys / keep_groups consecutive keys (one per view; non-zero: kept); a key that is not kept is not read.  A query without any
+ * kept key gets 0 and passes no gradient on. */
+typedef struct mvr_attend_params {
+  int32_t batch, queries, keys, heads, kv_heads, dim;
+  int32_t type;            /* MVR_TYPE_HALF or MVR_TYPE_BFLOAT: of every tensor but lse */
+  int32_t keep_groups;     /* 0: no mask */
+  int64_t q_stride[3], k_stride[3], v_stride[3];   /* in elements: batch, token, head; a head's elements are contiguous */
+  int64_t grad_stride[3];  /* of grad_out, the same (backward only) */
+  float scale;             /* > 0 */
+  int32_t reserved_;       /* explicit padding; must be 0 */
+} mvr_attend_params;
+
+size_t mvr_attend_tokens_workspace_bytes(const mvr_attend_params *params, int32_t backward);
+/* out: (batch, queries, heads, dim) contiguous.  lse: (batch, heads, queries) f32 for the backward, or NULL.  The workspace
+ * may be NULL where 0 bytes are asked for. */
+int mvr_attend_tokens_forward(const mvr_attend_params *params, const void *q, const void *k, const void *v, const uint8_t *keep,
+                              void *out, float *lse, void *workspace, size_t workspace_bytes, mvr_stream_t stream);
+/* out, lse: of the forward.  Gradients: contiguous, shaped as q, k, v.  Sums are taken in a fixed order (bit-reproducible). */
+int mvr_attend_tokens_backward(const mvr_attend_params *params, const void *q, const void *k, const void *v,
+                               const uint8_t *keep, const void *out, const float *lse, const void *grad_out, void *grad_q,
+                               void *grad_k, void *grad_v, void *workspace, size_t workspace_bytes, mvr_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -74,11 +74,19 @@ class NormParams(ctypes.Structure):  # struct mvr_norm_params
                 ("scale_groups", ctypes.c_int64), ("scale", ctypes.c_float), ("eps", ctypes.c_float)]
 
 
+class AttendParams(ctypes.Structure):  # struct mvr_attend_params
+    _fields_ = [(n, ctypes.c_int32) for n in ("batch", "queries", "keys", "heads", "kv_heads", "dim", "type", "keep_groups")] + [
+        (n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride", "grad_stride")] + [("scale", ctypes.c_float), ("reserved_", ctypes.c_int32)]
+
+
 # name -> (restype, argtypes); mirrors include/mvr.h one to one
 _MB, _MP, _PP = ctypes.POINTER(MeshBatch), ctypes.POINTER(MeshParams), ctypes.POINTER(PointsParams)
 _PL = ctypes.POINTER(PackLayout)
-_RP, _NP = ctypes.POINTER(RotaryParams), ctypes.POINTER(NormParams)
+_RP, _NP, _AP = ctypes.POINTER(RotaryParams), ctypes.POINTER(NormParams), ctypes.POINTER(AttendParams)
 PROTOTYPES = {
+    "mvr_attend_tokens_workspace_bytes": (ctypes.c_size_t, [_AP, ctypes.c_int32]),
+    "mvr_attend_tokens_forward": (ctypes.c_int, [_AP] + [_vp] * 7 + [ctypes.c_size_t, _vp]),
+    "mvr_attend_tokens_backward": (ctypes.c_int, [_AP] + [_vp] * 11 + [ctypes.c_size_t, _vp]),
     "mvr_rotate_tokens_forward": (ctypes.c_int, [_RP] + [_vp] * 5),
     "mvr_rotate_tokens_backward": (ctypes.c_int, [_RP] + [_vp] * 7),
     "mvr_add_norm_tokens_forward": (ctypes.c_int, [_NP] + [_vp] * 11),

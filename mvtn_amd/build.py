@@ -46,7 +46,7 @@ def _sources():
 
 
 def _token_sources():
-    return [os.path.join(CSRC, "mvr_tokens.hip")]
+    return [os.path.join(CSRC, "mvr_tokens.hip"), os.path.join(CSRC, "mvr_attend.hip")]
 
 
 def _src_hash(srcs, flags):

@@ -162,6 +162,93 @@ class _Rotate(torch.autograd.Function):
 
 
 # ---------------------------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------------------------
+
+def attend_tokens(q, k, v, keep=None, scale=None):
+    """softmax(scale q k^T) v over the kept keys: q (B, Lq, H, D), k and v (B, Lk, Hkv, D) float16 or bfloat16, D at most 128, H a multiple of
+    Hkv (consecutive heads share a key/value head); any strides whose last dimension is contiguous.  scale: D ** -0.5 by default.
+
+    keep: (B, G) with G a divisor of Lk, non-zero where the Lk / G consecutive keys of a group stay — one entry per key, or one per view
+    (`draw_regularization`'s scale, viewed as (B, V)).  Keys that are left out are not read and get gradient 0; a query without any key
+    left gets 0.  Returns (B, Lq, H, D), differentiable with respect to q, k and v: the backward recomputes the probabilities."""
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
+        raise ValueError("q is (B, Lq, H, D), k and v are (B, Lk, Hkv, D)")
+    B, Lq, H, D = q.shape
+    Lk, E = k.shape[1:3]
+    if k.shape[0] != B or k.shape[3] != D or not 1 <= D <= 128:
+        raise ValueError("q, k and v share the batch and a head size of 1 to 128")
+    if E < 1 or H < 1 or H % E:
+        raise ValueError("%d heads are not a multiple of %d key/value heads" % (H, E))
+    if q.dtype not in (torch.float16, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("q, k and v share one type of float16, bfloat16")
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0 < scale < math.inf:
+        raise ValueError("scale must be positive and finite")
+    if keep is not None:
+        if keep.dim() != 2 or keep.shape[0] != B or keep.shape[1] < 1 or Lk % keep.shape[1]:
+            raise ValueError("keep is (B, G) with G a divisor of the %d keys" % Lk)
+        if keep.requires_grad:
+            raise ValueError("keep is a mask: it gets no gradient")
+    _same_device(q, k, v, keep)
+    if keep is not None:
+        keep = (keep if keep.dtype in (torch.bool, torch.uint8) else keep != 0).contiguous()
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _Attend.apply(q, k, v, keep, scale)
+    return _attend(q, k, v, keep, scale, False)[0]
+
+
+def _attend_params(q, k, v, keep, scale):
+    B, Lq, H, D = q.shape
+    p = _lib.AttendParams(B, Lq, k.shape[1], H, k.shape[2], D, _TYPES[q.dtype], 0 if keep is None else keep.shape[1])
+    p.q_stride, p.k_stride, p.v_stride, p.scale = q.stride()[:3], k.stride()[:3], v.stride()[:3], scale
+    return p
+
+
+def _attend(q, k, v, keep, scale, training):
+    q, k, v = _rows_contiguous(q), _rows_contiguous(k), _rows_contiguous(v)
+    B, Lq, H, D = q.shape
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty(B, H, Lq, dtype=torch.float32, device=q.device) if training else None
+    if k.shape[1] == 0:
+        out.zero_()
+    elif out.numel():
+        params = _attend_params(q, k, v, keep, scale)
+        size = _lib.load().mvr_attend_tokens_workspace_bytes(params, 0)
+        ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+        _call("mvr_attend_tokens_forward", q.device, params, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(keep), out.data_ptr(), _ptr(lse),
+              _ptr(ws), size)
+    return out, (q, k, v, keep, out, lse)
+
+
+class _Attend(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, keep, scale):
+        out, kept = _attend(q, k, v, keep, scale, True)
+        ctx.scale = scale
+        ctx.save_for_backward(*kept)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        q, k, v, keep, out, lse = ctx.saved_tensors
+        gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        if out.numel() and k.shape[1]:
+            grad = _rows_contiguous(grad)
+            params = _attend_params(q, k, v, keep, ctx.scale)
+            params.grad_stride = grad.stride()[:3]
+            size = _lib.load().mvr_attend_tokens_workspace_bytes(params, 1)
+            ws = torch.empty(size, dtype=torch.uint8, device=q.device)
+            _call("mvr_attend_tokens_backward", q.device, params, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(keep), out.data_ptr(),
+                  lse.data_ptr(), grad.data_ptr(), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), ws.data_ptr(), size)
+        else:
+            for t in (gq, gk, gv):
+                t.zero_()
+        return gq, gk, gv, None, None
+
+
+# ---------------------------------------------------------------------------------------------
 # norms around a block
 # ---------------------------------------------------------------------------------------------
 

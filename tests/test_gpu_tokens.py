@@ -308,3 +308,90 @@ def test_rotary_and_norm_on_another_stream_and_in_a_graph():
         eager = step(xk)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, eager)), k
+
+
+# ---- attention -------------------------------------------------------------------------------------------------------
+
+def _attend64(q, k, v, keep, scale, do):
+    """o, dq, dk, dv in 64 bits over the kept keys only, and the absolute sums that enter the rounding of P and dS: see the test."""
+    B, Lq, H, D = q.shape
+    Lk, E = k.shape[1:3]
+    out = [torch.zeros(t.shape, dtype=torch.float64, device=q.device) for t in (q, q, k, v)]
+    size = [torch.zeros_like(t) for t in out]
+    for b in range(B):
+        on = torch.ones(Lk, dtype=torch.bool, device=q.device) if keep is None else (keep[b] != 0).repeat_interleave(Lk // keep.shape[1])
+        at = on.nonzero()[:, 0]
+        if not at.numel():
+            continue
+        for h in range(H):
+            e = h // (H // E)
+            Q, G = q[b, :, h].double(), do[b, :, h].double()
+            K, V = k[b, at, e].double(), v[b, at, e].double()
+            p = torch.softmax(Q @ K.T * scale, -1)
+            o, dp = p @ V, G @ V.T
+            ds = p * (dp - (G * o).sum(-1, keepdim=True))
+            # |dS| with its two parts apart: p |dp| + p |delta|, where delta comes from the stored o
+            ads = p * (dp.abs() + (G.abs() * o.abs()).sum(-1, keepdim=True))
+            out[0][b, :, h], out[1][b, :, h] = o, ds @ K * scale
+            size[0][b, :, h], size[1][b, :, h] = p @ V.abs(), ads @ K.abs() * scale
+            out[2][b, at, e] += ds.T @ Q * scale
+            out[3][b, at, e] += p.T @ G
+            size[2][b, at, e] += ads.T @ Q.abs() * scale
+            size[3][b, at, e] += p.T @ G.abs()
+    return out, size
+
+
+ATTENTION = [
+    # B, Lq, Lk, H, E, D, groups, dropped
+    (1, 1, 1, 1, 1, 1, 0, 0.0),                  # the smallest
+    (2, 12, 12, 12, 12, 64, 12, 0.5),            # a token per view
+    (3, 31, 33, 2, 2, 32, 0, 0.0),
+    (2, 64, 64, 3, 3, 64, 0, 0.0),               # whole tiles
+    (2, 65, 127, 4, 2, 40, 0, 0.0),              # ragged tiles, shared heads
+    (1, 196, 196, 3, 1, 64, 4, 0.5),             # views of 49 tokens: groups end inside tiles
+    (2, 5, 300, 6, 3, 96, 20, 0.3),
+    (2, 129, 260, 2, 1, 128, 260, 0.4),          # a mask of single keys
+    (2, 1, 1000, 8, 2, 128, 20, 0.25),           # one query: the keys are split
+    (1, 1, 4500, 2, 2, 72, 0, 0.0),              # more tiles than a mask chunk
+    (1, 3, 9000, 1, 1, 33, 9000, 0.9),           # odd head, most keys gone, three chunks
+    (2, 300, 1, 2, 2, 17, 0, 0.0),               # one key
+    (1, 700, 50, 4, 1, 104, 2, 0.5),             # many rows over few keys
+    (2, 40, 640, 2, 2, 64, 5, 0.99),             # objects with every view dropped
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,Lq,Lk,H,E,D,groups,dropped", ATTENTION)
+def test_attention_matches_the_definition(dtype, B, Lq, Lk, H, E, D, groups, dropped):
+    g = _gen(Lq * 7 + Lk)
+    q, k, v, do = (_randn(g, *s, dtype=dtype) for s in ((B, Lq, H, D), (B, Lk, E, D), (B, Lk, E, D), (B, Lq, H, D)))
+    keep = None
+    if groups:
+        keep = torch.rand(B, groups, generator=g, device=_dev()) >= dropped
+        if dropped > 0.9:
+            keep[-1] = False
+    want, size = _attend64(q, k, v, keep, D ** -0.5, do)
+    if groups:   # what a dropped key holds stays out
+        gone = ~keep.repeat_interleave(Lk // groups, 1)
+        k[gone], v[gone] = math.nan, math.inf
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = tokens.attend_tokens(*leaves, keep=keep)
+    got = [out.detach()] + list(torch.autograd.grad(out, leaves, do))
+    # scores: D products summed in 32 bits, |s log2 e| <= ~ 1.5 |q||k| / sqrt(D): exp2 moves by ln 2 times that error: bounded by 2^-24 (D + 8)
+    # times the score's size, far below u(dtype) here.  P and dS are each rounded once (u) against their own absolute size, delta carries the
+    # stored output's rounding (u); then the store (u).  1/32 u more for the 32-bit arithmetic (D and Lk sums: at most ~ 1e3 2^-24).
+    u = _u(dtype)
+    room = (1 + 1 / 32) * u + 2 ** -24 * (4 * D + 64)
+    for name, a, w, s, inner in zip(("out", "dq", "dk", "dv"), got, want, size, (1, 2, 2, 1)):
+        assert torch.isfinite(a).all(), name
+        # subnormal steps of float16 in P and dS: below 2^-14 a value is off by up to 2^-25, times at most Lk or the rows, times |k|, |q|, |do| < 6
+        low = 2 ** -25 * 6 * max(Lk, Lq * (H // E)) * D ** -0.5 if dtype == torch.float16 and name in ("dq", "dk") else 2 ** -25 * 6 * max(Lk, Lq * (H // E)) if dtype == torch.float16 else 0.0
+        assert ((a.double() - w).abs() <= room * w.abs() + inner * room * s + low + 1e-30).all(), (name, float((a.double() - w).abs().max()))
+    if groups:
+        assert not got[2][gone].any() and not got[3][gone].any()
+        empty = ~keep.any(1)
+        assert not got[0][empty].any() and not got[1][empty].any()
+    again = torch.autograd.grad(tokens.attend_tokens(*leaves, keep=keep), leaves, do)
+    assert all(torch.equal(a, b) for a, b in zip(again, got[1:]))   # bit-reproducible
+    with torch.no_grad():
+        assert torch.equal(tokens.attend_tokens(*leaves, keep=keep), got[0])

@@ -120,3 +120,48 @@ def test_c_abi_refuses_before_any_launch():
     assert backward(norm(), gw=p) == 3 and backward(norm(), gw=p, ws=p, size=need - 1) == 3
     assert backward(norm(), gy=None) == 1 and backward(norm(), gg=p) == 1 and backward(norm(), gp=p) == 1
     assert lib.mvr_add_norm_tokens_forward(None, p, p, p, None, None, None, None, p, p, None, None) == 1
+
+
+def test_attention_refuses_bad_calls():
+    f, half = tokens.attend_tokens, torch.float16
+    q = lambda *s, dtype=half: _x(*s, dtype=dtype)  # noqa: E731
+    ok = (q(2, 3, 4, 8), q(2, 6, 2, 8), q(2, 6, 2, 8))
+    for args, kw in (((q(2, 3, 8),) + ok[1:], {}), ((ok[0], ok[1], q(2, 5, 2, 8)), {}), ((ok[0], q(1, 6, 2, 8), q(1, 6, 2, 8)), {}),
+                     ((ok[0], q(2, 6, 3, 8), q(2, 6, 3, 8)), {}), ((q(2, 3, 4, 129), q(2, 6, 2, 129), q(2, 6, 2, 129)), {}),
+                     ((ok[0].float(), ok[1].float(), ok[2].float()), {}), ((ok[0], ok[1].bfloat16(), ok[2]), {}), (ok, dict(scale=0.0)), (ok, dict(scale=-1.0)),
+                     (ok, dict(scale=math.nan)), (ok, dict(scale=math.inf)), (ok, dict(keep=_x(2, 4))), (ok, dict(keep=_x(1, 6))), (ok, dict(keep=_x(2, 0))),
+                     (ok, dict(keep=_x(6))), (ok, dict(keep=_x(2, 6).requires_grad_())), ((q(2, 3, 4, 0), q(2, 6, 2, 0), q(2, 6, 2, 0)), {}),
+                     ((ok[0], q(2, 6, 0, 8), q(2, 6, 0, 8)), {})):
+        with pytest.raises(ValueError):
+            f(*args, **kw)
+    with pytest.raises(RuntimeError, match="GPU"):
+        f(*ok)
+
+
+def test_attention_c_abi_refuses_before_any_launch():
+    lib = _lib.load()
+    p = 4096
+
+    def params(**kw):
+        r = _lib.AttendParams(2, 3, 6, 4, 2, 8, 1, 0)
+        r.scale = 1.0
+        for k, v in kw.items():
+            setattr(r, k, v)
+        return r
+
+    def forward(a, keep=None, out=p + 64, ws=None, size=0):
+        return lib.mvr_attend_tokens_forward(a, p, p, p, keep, out, None, ws, size, None)
+
+    def backward(a, ws=p, size=1 << 40, gq=p, keep=None):
+        return lib.mvr_attend_tokens_backward(a, p, p, p, keep, p, p, p, gq, p, p, ws, size, None)
+    for kw, code in ((dict(batch=0), 1), (dict(queries=0), 1), (dict(keys=-5), 1), (dict(heads=3), 1), (dict(kv_heads=0), 1), (dict(dim=0), 1), (dict(dim=129), 4),
+                     (dict(type=0), 4), (dict(type=7), 4), (dict(keep_groups=4), 1), (dict(keep_groups=-1), 1), (dict(scale=0.0), 1), (dict(scale=math.nan), 1),
+                     (dict(scale=math.inf), 1), (dict(reserved_=1), 1), (dict(keys=0x7FFFFFFF), 4), (dict(queries=0x7FFFFFFF, heads=4), 4)):
+        assert forward(params(**kw)) == code and backward(params(**kw)) == code and lib.mvr_attend_tokens_workspace_bytes(params(**kw), 1) == 0, kw
+        assert b"mvr_attend_tokens" in lib.mvr_last_error()
+    assert forward(params(keep_groups=2)) == 1 and forward(params(), keep=p) == 1 and backward(params(), keep=p) == 1
+    assert forward(params(), out=p) == 1 and backward(params(), gq=None) == 1
+    assert backward(params(), ws=None) == 3 and backward(params(), size=lib.mvr_attend_tokens_workspace_bytes(params(), 1) - 1) == 3
+    split = params(batch=1, queries=1, keys=4096, heads=2)   # few rows: the keys are split and the parts need room
+    need = lib.mvr_attend_tokens_workspace_bytes(split, 0)
+    assert need > 0 and forward(split, ws=p, size=need - 1) == 3 and lib.mvr_attend_tokens_workspace_bytes(params(), 0) == 0
