@@ -53,13 +53,6 @@ struct AttArgs {
   float c, scale;                // scale log2(e)
 };
 
-// LDS only: global loads that are in flight for the next tile stay in flight
-__device__ __forceinline__ void lds_barrier() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
-
 // Workgroups are dealt to the 8 XCDs round robin: item = a contiguous run of the work per XCD, so that the workgroups which read one
 // object's keys share an L2
 __device__ __forceinline__ int64_t work_item(int64_t work) {

@@ -27,19 +27,47 @@ inline int launched(const char *what) {
   return fail(MVR_ERR_HIP, buf);
 }
 
-// N consecutive elements as 32-bit floats.  Whole vectors go through memcpy: one or two 16-byte accesses whatever the alignment (rows of odd
+// N consecutive elements on their way.  Whole vectors go through memcpy: 8- and 16-byte accesses whatever the alignment (rows of odd
 // width start anywhere; the hardware takes unaligned vector accesses), the last vector of such a row element by element.
+template <typename T, int N>
+struct Raw {
+  static constexpr int kWords = N * (int)sizeof(T) / 4;   // kept as words: 16-bit elements on their way take half a register each
+  unsigned w[kWords];
+  __device__ __forceinline__ void load(const T *p, int left) {
+    if (left >= N) {
+      __builtin_memcpy(w, p, sizeof w);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kWords; ++k) w[k] = 0;
+      const unsigned short *h = reinterpret_cast<const unsigned short *>(p);
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+          if (k < left) __builtin_memcpy(&w[k], p + k, 4);
+      } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+          if (k < left) w[k / 2] |= (unsigned)h[k] << (16 * (k & 1));
+      }
+    }
+  }
+  __device__ __forceinline__ void get(float (&v)[N]) const {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      if constexpr (sizeof(T) == 4) {
+        v[k] = __builtin_bit_cast(float, w[k]);
+      } else {
+        const unsigned short h = (unsigned short)(w[k / 2] >> (16 * (k & 1)));
+        v[k] = (float)__builtin_bit_cast(T, h);
+      }
+    }
+  }
+};
 template <int N, typename T>
 __device__ __forceinline__ void load_n(const T *p, int left, float (&v)[N]) {
-  if (left >= N) {
-    T t[N];
-    __builtin_memcpy(t, p, sizeof t);
-#pragma unroll
-    for (int k = 0; k < N; ++k) v[k] = (float)t[k];
-  } else {
-#pragma unroll
-    for (int k = 0; k < N; ++k) v[k] = k < left ? (float)p[k] : 0.0f;
-  }
+  Raw<T, N> r;
+  r.load(p, left);
+  r.get(v);
 }
 template <int N, typename T>
 __device__ __forceinline__ void store_n(T *p, int left, const float (&v)[N]) {
@@ -53,6 +81,13 @@ __device__ __forceinline__ void store_n(T *p, int left, const float (&v)[N]) {
     for (int k = 0; k < N; ++k)
       if (k < left) p[k] = (T)v[k];
   }
+}
+
+// a barrier that waits for LDS only: global loads in flight stay in flight
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
 template <int CTRL>

@@ -45,88 +45,105 @@ template <typename T, bool INTER, bool BWD, bool GPOS>
 __global__ __launch_bounds__(kBlock) void k_rotate_tokens(RotArgs a) {
   constexpr int VE = 16 / sizeof(T);            // elements of a unit's vector
   constexpr int NP = INTER ? VE / 2 : VE;       // pairs of a unit
+  constexpr int AHEAD = GPOS ? 2 : 4;           // heads whose loads are in flight
   extern __shared__ float2 cs[];                // [tb][n]; then, with GPOS, the slopes [hs][tb][n] as floats
   const int tid = threadIdx.x;
-  const int64_t row0 = (int64_t)blockIdx.x * a.tb;
-  const int here = (int)(a.rows - row0 < a.tb ? a.rows - row0 : a.tb);
+  const unsigned row0 = blockIdx.x * (unsigned)a.tb, rows = (unsigned)a.rows, L = (unsigned)a.L;
+  const int here = (int)(rows - row0 < (unsigned)a.tb ? rows - row0 : (unsigned)a.tb);
+  float *slopes = reinterpret_cast<float *>(cs + a.tb * a.n);
+  const int u = tid % a.rest, q = tid / a.rest, slice = q % a.hs, t = q / a.hs;
+  const bool live = t < here, turned = live && u < a.units;
+  const unsigned row = row0 + (live ? t : 0), b = row / L, l = row - b * L;
+  const T *in = (const T *)(BWD ? a.g : a.x) + (BWD ? b * a.gs[0] + l * a.gs[1] : b * a.xs[0] + l * a.xs[1]);
+  const int64_t in_h = BWD ? a.gs[2] : a.xs[2];
+  const T *x = GPOS ? (const T *)a.x + b * a.xs[0] + l * a.xs[1] : nullptr;
+  T *out = (T *)a.out + (int64_t)row * a.H * a.D;
+  const int i0 = u * NP;                        // first pair
+  // where the unit's vectors lie in a head, and how much of them is there
+  const int at1 = INTER ? 2 * i0 : i0, at2 = a.n + i0;
+  const int left = INTER ? a.D - at1 : a.n - i0;
+  const int pairs = a.n - i0;                   // pairs behind it (interleaved: the head's tail in this vector) stay as they are
+  Raw<T, VE> v1[AHEAD], v2[AHEAD], x1[AHEAD], x2[AHEAD];
+  const auto fetch = [&](int j, int h) {
+    v1[j].load(in + h * in_h + at1, left);
+    if constexpr (!INTER) v2[j].load(in + h * in_h + at2, left);
+    if constexpr (GPOS) {
+      x1[j].load(x + h * a.xs[2] + at1, left);
+      if constexpr (!INTER) x2[j].load(x + h * a.xs[2] + at2, left);
+    }
+  };
+  if (turned) {
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+      if (slice + j * a.hs < a.H) fetch(j, slice + j * a.hs);
+  }
+  // the angles, while the first heads are on their way
   for (int e = tid; e < here * a.n; e += kBlock) {
-    const int t = e / a.n, i = e - t * a.n;
+    const int t1 = e / a.n, i = e - t1 * a.n;
     int axis = 0;
     for (int k = 0; k + 1 < a.axes; ++k) axis += i >= a.end[k];
-    const int64_t row = row0 + t, b = row / a.L, l = row - b * a.L;
-    const double p = (double)a.pos[b * a.ps[0] + l * a.ps[1] + axis] * a.turns[i];
+    const unsigned r1 = row0 + t1, b1 = r1 / L, l1 = r1 - b1 * L;
+    const double p = (double)a.pos[b1 * a.ps[0] + l1 * a.ps[1] + axis] * a.turns[i];
     const float r = (float)(p - rint(p));
     float s, c;
     sincospif(2.0f * r, &s, &c);
     cs[e] = make_float2(c, BWD ? -s : s);
   }
-  __syncthreads();
-  float *slopes = reinterpret_cast<float *>(cs + a.tb * a.n);
-  const int u = tid % a.rest, q = tid / a.rest, t = q % a.tb, slice = q / a.tb;
-  if (slice < a.hs && t < here) {
-    const int64_t row = row0 + t, b = row / a.L, l = row - b * a.L;
-    const T *in = (const T *)(BWD ? a.g : a.x) + (BWD ? b * a.gs[0] + l * a.gs[1] : b * a.xs[0] + l * a.xs[1]);
-    const int64_t in_h = BWD ? a.gs[2] : a.xs[2];
-    const T *x = (const T *)a.x + (GPOS ? b * a.xs[0] + l * a.xs[1] : 0);
-    T *out = (T *)a.out + row * a.H * a.D;
-    if (u < a.units) {
-      const int i0 = u * NP;                    // first pair
-      float c[NP], s[NP], th[NP];
+  lds_barrier();
+  if (turned) {
+    float c[NP], s[NP], th[NP];
 #pragma unroll
-      for (int k = 0; k < NP; ++k) {
-        const bool on = i0 + k < a.n;
-        const float2 v = on ? cs[t * a.n + i0 + k] : make_float2(1.0f, 0.0f);
-        c[k] = v.x, s[k] = v.y, th[k] = 0.0f;
-      }
-      // where the unit's vectors lie in a head, and how much of them is there
-      const int at1 = INTER ? 2 * i0 : i0, at2 = a.n + i0;
-      const int left = INTER ? a.D - at1 : a.n - i0;
-      const int live = a.n - i0;                // pairs behind it (interleaved: the head's tail in this vector) stay as they are
-#pragma unroll 4
-      for (int h = slice; h < a.H; h += a.hs) {
-        const T *p = in + h * in_h;
-        T *o = out + (int64_t)h * a.D;
+    for (int k = 0; k < NP; ++k) {
+      const float2 v = k < pairs ? cs[t * a.n + i0 + k] : make_float2(1.0f, 0.0f);
+      c[k] = v.x, s[k] = v.y, th[k] = 0.0f;
+    }
+    for (int h0 = slice; h0 < a.H; h0 += a.hs * AHEAD) {
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const int h = h0 + j * a.hs, next = h + a.hs * AHEAD;
+        if (h >= a.H) break;
         float v[VE], w[VE], xv[VE], xw[VE];
-        load_n<VE>(p + at1, left, v);
-        if constexpr (!INTER) load_n<VE>(p + at2, left, w);
+        v1[j].get(v);
+        if constexpr (!INTER) v2[j].get(w);
         if constexpr (GPOS) {
-          load_n<VE>(x + h * a.xs[2] + at1, left, xv);
-          if constexpr (!INTER) load_n<VE>(x + h * a.xs[2] + at2, left, xw);
+          x1[j].get(xv);
+          if constexpr (!INTER) x2[j].get(xw);
         }
+        if (next < a.H) fetch(j, next);
 #pragma unroll
         for (int k = 0; k < NP; ++k) {
           const float e1 = INTER ? v[2 * k] : v[k], e2 = INTER ? v[2 * k + 1] : w[k];
           const float r1 = e1 * c[k] - e2 * s[k], r2 = e1 * s[k] + e2 * c[k];
           if constexpr (GPOS) {
-            const float x1 = INTER ? xv[2 * k] : xv[k], x2 = INTER ? xv[2 * k + 1] : xw[k];
-            th[k] += k < live ? x1 * r2 - x2 * r1 : 0.0f;
+            const float p1 = INTER ? xv[2 * k] : xv[k], p2 = INTER ? xv[2 * k + 1] : xw[k];
+            th[k] += k < pairs ? p1 * r2 - p2 * r1 : 0.0f;
           }
           if constexpr (INTER) {
-            v[2 * k] = k < live ? r1 : e1;
-            v[2 * k + 1] = k < live ? r2 : e2;
+            v[2 * k] = k < pairs ? r1 : e1;
+            v[2 * k + 1] = k < pairs ? r2 : e2;
           } else {
             v[k] = r1, w[k] = r2;
           }
         }
-        store_n<VE>(o + at1, left, v);
-        if constexpr (!INTER) store_n<VE>(o + at2, left, w);
+        store_n<VE>(out + (int64_t)h * a.D + at1, left, v);
+        if constexpr (!INTER) store_n<VE>(out + (int64_t)h * a.D + at2, left, w);
       }
-      if constexpr (GPOS) {
+    }
+    if constexpr (GPOS) {
 #pragma unroll
-        for (int k = 0; k < NP; ++k)
-          if (k < live) slopes[(slice * a.tb + t) * a.n + i0 + k] = th[k];
-      }
-    } else {                                    // the head's part behind the pairs
-      const int at = (INTER ? a.units * VE : 2 * a.n) + (u - a.units) * VE;
-      for (int h = slice; h < a.H; h += a.hs) {
-        float v[VE];
-        load_n<VE>(in + h * in_h + at, a.D - at, v);
-        store_n<VE>(out + (int64_t)h * a.D + at, a.D - at, v);
-      }
+      for (int k = 0; k < NP; ++k)
+        if (k < pairs) slopes[(slice * a.tb + t) * a.n + i0 + k] = th[k];
+    }
+  } else if (live) {                            // the head's part behind the pairs
+    const int at = (INTER ? a.units * VE : 2 * a.n) + (u - a.units) * VE;
+    for (int h = slice; h < a.H; h += a.hs) {
+      float v[VE];
+      load_n<VE>(in + h * in_h + at, a.D - at, v);
+      store_n<VE>(out + (int64_t)h * a.D + at, a.D - at, v);
     }
   }
   if constexpr (GPOS) {
-    __syncthreads();
+    lds_barrier();
     for (int e = tid; e < here * a.axes; e += kBlock) {
       const int t1 = e / a.axes, ax = e - t1 * a.axes;
       float sum = 0.0f;
@@ -135,7 +152,7 @@ __global__ __launch_bounds__(kBlock) void k_rotate_tokens(RotArgs a) {
         for (int k = 0; k < a.hs; ++k) th += slopes[(k * a.tb + t1) * a.n + i];
         sum += th * (float)(2.0 * M_PI * a.turns[i]);
       }
-      a.gpos[(row0 + t1) * a.axes + ax] = sum;
+      a.gpos[(int64_t)(row0 + t1) * a.axes + ax] = sum;
     }
   }
 }
@@ -159,6 +176,7 @@ int rotary_args(RotArgs &a, const mvr_rotary_params *p, const double *turns) {
   if (p->interleaved && p->dim % 2) return bad("mvr_rotate_tokens: interleaved pairs need an even head dimension");
   const int ve = 16 / type_size(p->type), np = p->interleaved ? ve / 2 : ve;
   a.rows = (int64_t)p->batch * p->tokens;
+  if (a.rows > 0x7FFFFFFF) return fail(MVR_ERR_UNSUPPORTED, "mvr_rotate_tokens: at most 2^31 - 1 tokens in a batch");
   a.L = p->tokens, a.H = p->heads, a.D = p->dim, a.n = n, a.axes = p->axes;
   for (int k = 0; k < 3; ++k) a.xs[k] = p->x_stride[k], a.gs[k] = p->grad_stride[k];
   a.ps[0] = p->position_stride[0], a.ps[1] = p->position_stride[1];
@@ -170,9 +188,10 @@ int rotary_args(RotArgs &a, const mvr_rotary_params *p, const double *turns) {
     a.units = (n + np - 1) / np;
     a.rest = a.units + (p->dim - 2 * n + ve - 1) / ve;
   }
-  // head slices: up to four threads share a (token, unit), so that a token's angles serve many heads and the workgroup still holds
-  // several tokens
-  a.hs = p->heads < 4 ? p->heads : 4;
+  // two heads a thread: both are on their way while the angles are formed, and a token's heads lie side by side in a wave's accesses
+  // (16 x 2352 x 24 heads x 64 bf16, forward / backward with the positions' gradient, us: one head 64 / 146, two 61 / 88, three 64 / 85,
+  // four 67 / 90, eight 72 / 94)
+  a.hs = (p->heads + 1) / 2;
   while (a.hs > 1 && a.rest * a.hs > kBlock) --a.hs;
   a.tb = kBlock / (a.rest * a.hs);
   if (a.tb > a.rows) a.tb = (int)a.rows;
@@ -184,7 +203,6 @@ int rotary_args(RotArgs &a, const mvr_rotary_params *p, const double *turns) {
 template <typename T>
 int launch_rotary_t(const RotArgs &a, bool inter, bool bwd, hipStream_t st) {
   const int64_t blocks = (a.rows + a.tb - 1) / a.tb;
-  if (blocks > 0x7FFFFFFF) return bad("mvr_rotate_tokens: too many tokens");
   const size_t lds = (size_t)a.tb * a.n * (sizeof(float2) + (a.gpos ? a.hs * sizeof(float) : 0));
   const dim3 g((unsigned)blocks), b(kBlock);
   if (!bwd) {
@@ -234,10 +252,12 @@ struct NormArgs {
   float s, eps;
 };
 
-__device__ __forceinline__ void load_param(const void *p, int type, int64_t at, int left, float (&v)[8]) {
-  if (type == MVR_TYPE_FLOAT) load_n<8>((const float *)p + at, left, v);
-  else if (type == MVR_TYPE_HALF) load_n<8>((const f16 *)p + at, left, v);
-  else load_n<8>((const bf16 *)p + at, left, v);
+constexpr int kV = 4;   // elements of a lane's vector
+
+__device__ __forceinline__ void load_param(const void *p, int type, int64_t at, int left, float (&v)[kV]) {
+  if (type == MVR_TYPE_FLOAT) load_n<kV>((const float *)p + at, left, v);
+  else if (type == MVR_TYPE_HALF) load_n<kV>((const f16 *)p + at, left, v);
+  else load_n<kV>((const bf16 *)p + at, left, v);
 }
 
 // sums over the row of K values at once; with WAVES > 1 through LDS, in wave order (two buffers: one barrier a call)
@@ -264,7 +284,7 @@ __device__ __forceinline__ void row_sum(float (&v)[K], float *lds, int &turn) {
 
 // mean (0 for rms) and 1 / std of a row held as v; places behind the row hold zeros and are left out of the second sum
 template <int WAVES, int NV>
-__device__ __forceinline__ float2 row_stats(const float (&v)[NV][8], const int (&left)[NV], const NormArgs &a, float *lds, int &turn) {
+__device__ __forceinline__ float2 row_stats(const float (&v)[NV][kV], const int (&left)[NV], const NormArgs &a, float *lds, int &turn) {
   float m = 0.0f;
   const float inv = 1.0f / (float)a.D;
   if (a.layer) {
@@ -272,7 +292,7 @@ __device__ __forceinline__ float2 row_stats(const float (&v)[NV][8], const int (
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) s[0] += v[j][k];
+      for (int k = 0; k < kV; ++k) s[0] += v[j][k];
     row_sum<WAVES>(s, lds, turn);
     m = s[0] * inv;
   }
@@ -280,7 +300,7 @@ __device__ __forceinline__ float2 row_stats(const float (&v)[NV][8], const int (
 #pragma unroll
   for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < kV; ++k) {
       const float d = k < left[j] ? v[j][k] - m : 0.0f;
       q[0] += d * d;
     }
@@ -288,137 +308,178 @@ __device__ __forceinline__ float2 row_stats(const float (&v)[NV][8], const int (
   return make_float2(m, 1.0f / sqrtf(q[0] * inv + a.eps));
 }
 
+// this wave's (workgroup's) rows: first, first + step, ...; the next row is on its way while one is worked on
 template <typename TR, typename TB, int WAVES, int NV>
-__global__ __launch_bounds__(kBlock) void k_add_norm(NormArgs a) {
-  __shared__ float lds[16];
+__global__ __launch_bounds__(WAVES > 1 ? 64 * WAVES : kBlock) void k_add_norm(NormArgs a) {
+  __shared__ float lds[4 * WAVES];
   int turn = 0;
   const int lane = WAVES > 1 ? threadIdx.x : threadIdx.x & 63;
   constexpr int kRows = WAVES > 1 ? 1 : kBlock / 64, kLanes = 64 * WAVES;
-  const int64_t step = (int64_t)gridDim.x * kRows;
-  int left[NV];
-  float w[NV][8], bi[NV][8], po[NV][8];
+  const unsigned rows = (unsigned)a.rows, step = gridDim.x * kRows, scale_rows = (unsigned)a.scale_rows, group_rows = (unsigned)a.group_rows;
+  int at[NV], left[NV];
+  float w[NV][kV], bi[NV][kV], po[NV][kV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int c = (lane + j * kLanes) * 8;
-    left[j] = a.D - c < 0 ? 0 : a.D - c;
-    load_param(a.weight, a.ptype, c, left[j], w[j]);
-    if (a.bias) load_param(a.bias, a.ptype, c, left[j], bi[j]);
-    if (a.post) load_param(a.post, a.ptype, c, left[j], po[j]);
+    at[j] = (lane + j * kLanes) * kV;
+    left[j] = a.D - at[j] < 0 ? 0 : a.D - at[j];
+    load_param(a.weight, a.ptype, at[j], left[j], w[j]);
+    if (a.bias) load_param(a.bias, a.ptype, at[j], left[j], bi[j]);
+    if (a.post) load_param(a.post, a.ptype, at[j], left[j], po[j]);
   }
-  for (int64_t row = (int64_t)blockIdx.x * kRows + (WAVES > 1 ? 0 : threadIdx.x / 64); row < a.rows; row += step) {
-    const TR *rp = (const TR *)a.residual + row * a.D;
-    const TB *bp = (const TB *)a.branch + row * a.D;
-    float v[NV][8], n[NV][8];
-    const float s = a.scale ? a.scale[row / a.scale_rows] : a.s;
-    const bool dropped = a.scale && s == 0.0f;   // a dropped view's branch is not read: whatever it holds stays out
+  Raw<TR, kV> rr[NV];
+  Raw<TB, kV> rb[NV];
+  float s = 0.0f;
+  bool dropped = false;
+  const auto fetch = [&](unsigned row) {
+    s = a.scale ? a.scale[row / scale_rows] : a.s;
+    dropped = a.scale && s == 0.0f;   // a dropped view's branch is not read: whatever it holds stays out
+    const TR *rp = (const TR *)a.residual + (int64_t)row * a.D;
+    const TB *bp = (const TB *)a.branch + (int64_t)row * a.D;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) rr[j].load(rp + at[j], left[j]), rb[j].load(bp + at[j], dropped ? 0 : left[j]);
+  };
+  unsigned row = __builtin_amdgcn_readfirstlane(blockIdx.x * kRows + (WAVES > 1 ? 0 : threadIdx.x / 64));
+  if (row < rows) fetch(row);
+  while (row < rows) {
+    float v[NV][kV], n[NV][kV], g[NV][kV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      load_n<8>(rp + (lane + j * kLanes) * 8, left[j], v[j]);
-      load_n<8>(bp + (lane + j * kLanes) * 8, dropped ? 0 : left[j], n[j]);
+      rr[j].get(v[j]), rb[j].get(n[j]);
+      if (a.gate) load_param(a.gate, a.ptype, (int64_t)(row / group_rows) * a.D + at[j], left[j], g[j]);
     }
+    const float s0 = s;
+    const bool gone = dropped;
+    const unsigned next = row + step;
+    if (next < rows) fetch(next);
     float2 sa = make_float2(0.0f, 1.0f);
     if (a.post) sa = row_stats<WAVES, NV>(n, left, a, lds, turn);
-    if (!dropped) {
+    if (!gone) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        float g[8];
-        if (a.gate) load_param(a.gate, a.ptype, (row / a.group_rows) * a.D + (lane + j * kLanes) * 8, left[j], g);
+      for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < kV; ++k) {
           float t = a.post ? (n[j][k] - sa.x) * sa.y * po[j][k] : n[j][k];
-          if (a.gate) t *= g[k];
-          if (k < left[j]) v[j][k] += s * t;
+          if (a.gate) t *= g[j][k];
+          if (k < left[j]) v[j][k] += s0 * t;
         }
-      }
     }
 #pragma unroll
-    for (int j = 0; j < NV; ++j) store_n<8>((TR *)a.y + row * a.D + (lane + j * kLanes) * 8, left[j], v[j]);
+    for (int j = 0; j < NV; ++j) store_n<kV>((TR *)a.y + (int64_t)row * a.D + at[j], left[j], v[j]);
     const float2 sy = row_stats<WAVES, NV>(v, left, a, lds, turn);
-    if (a.stats && lane == 0) *reinterpret_cast<float4 *>(a.stats + row * 4) = make_float4(sy.x, sy.y, sa.x, sa.y);
+    if (a.stats && lane == 0) *reinterpret_cast<float4 *>(a.stats + (int64_t)row * 4) = make_float4(sy.x, sy.y, sa.x, sa.y);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < kV; ++k) {
         v[j][k] = (v[j][k] - sy.x) * sy.y * w[j][k];
         if (a.bias) v[j][k] += bi[j][k];
       }
-      store_n<8>((TB *)a.z + row * a.D + (lane + j * kLanes) * 8, left[j], v[j]);
+      store_n<kV>((TB *)a.z + (int64_t)row * a.D + at[j], left[j], v[j]);
     }
+    row = next;
   }
 }
 
 template <typename TR, typename TB, int WAVES, int NV>
-__global__ __launch_bounds__(kBlock) void k_add_norm_backward(NormArgs a) {
+__global__ __launch_bounds__(WAVES > 1 ? 64 * WAVES : kBlock) void k_add_norm_backward(NormArgs a) {
   constexpr int kRows = WAVES > 1 ? 1 : kBlock / 64, kLanes = 64 * WAVES;
-  __shared__ float lds[16];
-  __shared__ float cols[WAVES > 1 ? 1 : kRows][WAVES > 1 ? 1 : kLanes * 8];
+  __shared__ float lds[4 * WAVES];
+  __shared__ float cols[WAVES > 1 ? 1 : kRows][WAVES > 1 ? 1 : kLanes * kV];
+  __shared__ float4 params[NV * kLanes][3];   // weight, post_weight, gate: in LDS, the registers go to rows and column sums
   int turn = 0;
-  const int lane = WAVES > 1 ? threadIdx.x : threadIdx.x & 63, wave = WAVES > 1 ? 0 : threadIdx.x / 64;
-  const int64_t group = blockIdx.x / a.blocks_per_group, part = blockIdx.x - group * a.blocks_per_group;
-  const int64_t first = group * a.group_rows + part * a.block_rows;
-  const int64_t end_g = (group + 1) * a.group_rows, last = first + a.block_rows < end_g ? first + a.block_rows : end_g;
+  const int lane = WAVES > 1 ? threadIdx.x : threadIdx.x & 63, wave = WAVES > 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const unsigned group = blockIdx.x / (unsigned)a.blocks_per_group, part = blockIdx.x - group * (unsigned)a.blocks_per_group;
+  const unsigned scale_rows = (unsigned)a.scale_rows, end_g = (group + 1) * (unsigned)a.group_rows;
+  const unsigned first = group * (unsigned)a.group_rows + part * (unsigned)a.block_rows;
+  const unsigned last = end_g - first < (unsigned)a.block_rows ? end_g : first + (unsigned)a.block_rows;
   const float inv = 1.0f / (float)a.D;
-  int left[NV];
-  float w[NV][8], po[NV][8], ga[NV][8];
-  float dw[NV][8], db[NV][8], dp[NV][8], dg[NV][8];
+  int at[NV], left[NV];
+  float dw[NV][kV], db[NV][kV], dp[NV][kV], dg[NV][kV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int c = (lane + j * kLanes) * 8;
-    left[j] = a.D - c < 0 ? 0 : a.D - c;
-    load_param(a.weight, a.ptype, c, left[j], w[j]);
-    if (a.post) load_param(a.post, a.ptype, c, left[j], po[j]);
-    if (a.gate) load_param(a.gate, a.ptype, group * a.D + c, left[j], ga[j]);
+    at[j] = (lane + j * kLanes) * kV;
+    left[j] = a.D - at[j] < 0 ? 0 : a.D - at[j];
+    float w[kV], po[kV], ga[kV];
+    load_param(a.weight, a.ptype, at[j], left[j], w);
+    if (a.post) load_param(a.post, a.ptype, at[j], left[j], po);
+    if (a.gate) load_param(a.gate, a.ptype, (int64_t)group * a.D + at[j], left[j], ga);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if (!a.post) po[j][k] = 1.0f;
-      if (!a.gate) ga[j][k] = 1.0f;
+    for (int k = 0; k < kV; ++k) {
+      if (!a.post) po[k] = 1.0f;
+      if (!a.gate) ga[k] = 1.0f;
       dw[j][k] = db[j][k] = dp[j][k] = dg[j][k] = 0.0f;
     }
+    // (all waves of a workgroup with rows of their own write the same values)
+    float4 *to = params[j * kLanes + lane];
+    to[0] = make_float4(w[0], w[1], w[2], w[3]), to[1] = make_float4(po[0], po[1], po[2], po[3]), to[2] = make_float4(ga[0], ga[1], ga[2], ga[3]);
   }
-  for (int64_t row = first + wave; row < last; row += kRows) {
-    const float s = a.scale ? a.scale[row / a.scale_rows] : a.s;
-    const bool dropped = a.scale && s == 0.0f;
-    const float4 st = *reinterpret_cast<const float4 *>(a.stats + row * 4);
-    float y[NV][8], n[NV][8], g[NV][8], t[NV][8];
+  lds_barrier();
+  Raw<TR, kV> ry[NV], rdy[NV];
+  Raw<TB, kV> rb[NV], rdz[NV];
+  float s = 0.0f;
+  bool dropped = false;
+  float4 stats;
+  const auto fetch = [&](unsigned row) {
+    s = a.scale ? a.scale[row / scale_rows] : a.s;
+    dropped = a.scale && s == 0.0f;
+    stats = *reinterpret_cast<const float4 *>(a.stats + (int64_t)row * 4);
+    const int64_t base = (int64_t)row * a.D;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int64_t at = row * a.D + (lane + j * kLanes) * 8;
-      load_n<8>((const TR *)a.residual + at, left[j], y[j]);
-      load_n<8>((const TB *)a.branch + at, dropped ? 0 : left[j], n[j]);
-      load_n<8>((const TB *)a.dz + at, a.dz ? left[j] : 0, g[j]);
-      load_n<8>((const TR *)a.dy + at, a.dy ? left[j] : 0, t[j]);
+      ry[j].load((const TR *)a.residual + base + at[j], left[j]);
+      rdz[j].load((const TB *)a.dz + base + at[j], a.dz ? left[j] : 0);
+      rdy[j].load((const TR *)a.dy + base + at[j], a.dy ? left[j] : 0);
+      rb[j].load((const TB *)a.branch + base + at[j], dropped ? 0 : left[j]);
     }
+  };
+  unsigned row = first + wave;
+  if (row < last) fetch(row);
+  while (row < last) {
+    asm volatile("" ::: "memory");   // (the parameters stay in LDS: hoisted out of the loop they cost a third of the registers)
+    float y[NV][kV], n[NV][kV], g[NV][kV], t[NV][kV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) ry[j].get(y[j]), rb[j].get(n[j]), rdz[j].get(g[j]), rdy[j].get(t[j]);
+    const float s0 = s;
+    const bool gone = dropped;
+    const float4 st = stats;
+    const unsigned next = row + kRows;
+    if (next < last) fetch(next);
     float m[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+    for (int j = 0; j < NV; ++j) {
+      const float4 w4 = params[j * kLanes + lane][0];
+      const float w[kV] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < kV; ++k) {
         y[j][k] = k < left[j] ? (y[j][k] - st.x) * st.y : 0.0f;   // yhat
         dw[j][k] += g[j][k] * y[j][k];
         db[j][k] += g[j][k];
-        g[j][k] *= w[j][k];
+        g[j][k] *= w[k];
         m[0] += g[j][k] * y[j][k];
         m[1] += g[j][k];
       }
+    }
     row_sum<WAVES>(m, lds, turn);
     const float m0 = m[0] * inv, m1 = a.layer ? m[1] * inv : 0.0f;
     float d[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
+      const float4 p4 = params[j * kLanes + lane][1], g4 = params[j * kLanes + lane][2];
+      const float po[kV] = {p4.x, p4.y, p4.z, p4.w}, ga[kV] = {g4.x, g4.y, g4.z, g4.w};
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < kV; ++k) {
         t[j][k] += st.y * (g[j][k] - m1 - y[j][k] * m0);          // dyt
-        const float hat = dropped || k >= left[j] ? 0.0f : a.post ? (n[j][k] - st.z) * st.w : n[j][k];
-        const float u = k < left[j] ? s * t[j][k] : 0.0f;
-        dg[j][k] += u * po[j][k] * hat;
-        const float dn = dropped ? 0.0f : u * ga[j][k];
+        const float hat = gone || k >= left[j] ? 0.0f : a.post ? (n[j][k] - st.z) * st.w : n[j][k];
+        const float u = k < left[j] ? s0 * t[j][k] : 0.0f;
+        dg[j][k] += u * po[k] * hat;
+        const float dn = gone ? 0.0f : u * ga[k];
         dp[j][k] += dn * hat;
         n[j][k] = hat;
-        g[j][k] = dn * po[j][k];
+        g[j][k] = dn * po[k];
         d[0] += g[j][k] * hat;
         d[1] += g[j][k];
       }
-      store_n<8>((TR *)a.dresidual + row * a.D + (lane + j * kLanes) * 8, left[j], t[j]);
+      store_n<kV>((TR *)a.dresidual + (int64_t)row * a.D + at[j], left[j], t[j]);
     }
     if (a.post) {
       row_sum<WAVES>(d, lds, turn);
@@ -426,10 +487,11 @@ __global__ __launch_bounds__(kBlock) void k_add_norm_backward(NormArgs a) {
 #pragma unroll
       for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) g[j][k] = dropped ? 0.0f : st.w * (g[j][k] - d1 - n[j][k] * d0);
+        for (int k = 0; k < kV; ++k) g[j][k] = gone ? 0.0f : st.w * (g[j][k] - d1 - n[j][k] * d0);
     }
 #pragma unroll
-    for (int j = 0; j < NV; ++j) store_n<8>((TB *)a.dbranch + row * a.D + (lane + j * kLanes) * 8, left[j], g[j]);
+    for (int j = 0; j < NV; ++j) store_n<kV>((TB *)a.dbranch + (int64_t)row * a.D + at[j], left[j], g[j]);
+    row = next;
   }
   if (!a.partial) return;
   float *line = a.partial + (int64_t)blockIdx.x * 4 * a.D;
@@ -437,38 +499,39 @@ __global__ __launch_bounds__(kBlock) void k_add_norm_backward(NormArgs a) {
   for (int q = 0; q < 4; ++q) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      float v[8];
+      float v[kV];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = q == 0 ? dw[j][k] : q == 1 ? db[j][k] : q == 2 ? dp[j][k] : dg[j][k];
+      for (int k = 0; k < kV; ++k) v[k] = q == 0 ? dw[j][k] : q == 1 ? db[j][k] : q == 2 ? dp[j][k] : dg[j][k];
       if constexpr (WAVES > 1) {
-        store_n<8>(line + q * a.D + (lane + j * kLanes) * 8, left[j], v);
+        store_n<kV>(line + q * a.D + at[j], left[j], v);
       } else {   // the four waves' rows, in wave order
-        __syncthreads();
+        lds_barrier();
 #pragma unroll
-        for (int k = 0; k < 8; ++k) cols[wave][lane + k * 64] = v[k];
-        __syncthreads();
-        for (int e = threadIdx.x; e < 512; e += kBlock) {
-          const int l = e >> 3, k = e & 7, c = (l + j * kLanes) * 8 + k;
-          if (c < a.D) line[q * a.D + c] = (cols[0][l + k * 64] + cols[1][l + k * 64]) + (cols[2][l + k * 64] + cols[3][l + k * 64]);
-        }
+        for (int k = 0; k < kV; ++k) cols[wave][lane * kV + k] = v[k];
+        lds_barrier();
+        const int e = threadIdx.x, c = j * kLanes * kV + e;
+        if (c < a.D) line[q * a.D + c] = (cols[0][e] + cols[1][e]) + (cols[2][e] + cols[3][e]);
       }
     }
   }
 }
 
 // 64 columns of one of the four sums: sixteen waves add the lines k, k + 16, ..., then wave 0 adds the waves' sums up
+constexpr int kColumns = 64;
 __global__ __launch_bounds__(1024) void k_norm_columns(const float *partial, int32_t D, int32_t blocks, int32_t blocks_per_group, int32_t ptype,
                                                        void *dweight, void *dbias, void *dpost, void *dgate) {
-  __shared__ float lds[16][64];
+  __shared__ float lds[16][kColumns];
   const int q = blockIdx.y < 3 ? blockIdx.y : 3;
   const int64_t group = blockIdx.y < 3 ? 0 : blockIdx.y - 3;
   void *out = q == 0 ? dweight : q == 1 ? dbias : q == 2 ? dpost : dgate;
   if (!out) return;
   const int first = q == 3 ? (int)group * blocks_per_group : 0, last = q == 3 ? first + blocks_per_group : blocks;
-  const int wave = threadIdx.x / 64, lane = threadIdx.x & 63, c = blockIdx.x * 64 + lane;
+  const int wave = threadIdx.x / kColumns, lane = threadIdx.x % kColumns, c = blockIdx.x * kColumns + lane;
   float s = 0.0f;
-  if (c < D)
+  if (c < D) {
+#pragma unroll 8
     for (int k = first + wave; k < last; k += 16) s += partial[((int64_t)k * 4 + q) * D + c];
+  }
   lds[wave][lane] = s;
   __syncthreads();
   if (wave == 0 && c < D) {
@@ -484,6 +547,7 @@ __global__ __launch_bounds__(1024) void k_norm_columns(const float *partial, int
 int norm_args(NormArgs &a, const mvr_norm_params *p) {
   if (!p) return bad("mvr_add_norm_tokens: params must be given");
   if (p->rows <= 0 || p->dim <= 0 || p->dim > 8192) return bad("mvr_add_norm_tokens: rows >= 1 and 1 <= dim <= 8192");
+  if (p->rows > 0x7FFF0000) return fail(MVR_ERR_UNSUPPORTED, "mvr_add_norm_tokens: too many rows");
   const int r = p->residual_type, b = p->branch_type;
   if (!type_size(r) || !type_size(b) || !type_size(p->param_type)) return bad("mvr_add_norm_tokens: unknown type");
   if (r != b && r != MVR_TYPE_FLOAT) return fail(MVR_ERR_UNSUPPORTED, "mvr_add_norm_tokens: the residual has the branch's type or 32 bits");
@@ -498,11 +562,23 @@ int norm_args(NormArgs &a, const mvr_norm_params *p) {
   return MVR_OK;
 }
 
-// Workgroups of the backward: about 1024 in all, each with a run of rows of one gate group
+// 256 elements of a row per wave and vector.  Rows of up to 768 lie in one wave's registers (16 x 2352 x 768 bf16, forward / backward: 55.5 / 78.6 us;
+// a row over the three waves of a workgroup: 69 / 82 with its columns); wider ones take a workgroup: 64 x 3920 x 1024 forward 586 us, with one
+// wave a row 622.
+// Grids hold as many workgroups as are resident at once (256 CUs by what the registers allow) and every wave runs through its rows: a second,
+// partly filled round costs more than it balances (backward at 768: 512 workgroups 79 us, 768 101, 1024 87).
+struct NormPlan { int32_t waves, vectors, forward, backward; };
+inline NormPlan norm_plan(int32_t D) {
+  return D <= 256 ? NormPlan{1, 1, 2048, 1280} : D <= 512 ? NormPlan{1, 2, 1280, 768} : D <= 768 ? NormPlan{1, 3, 1024, 512}
+         : D <= 1024 ? NormPlan{4, 1, 2048, 768} : D <= 2048 ? NormPlan{4, 2, 1280, 768} : D <= 4096 ? NormPlan{8, 2, 512, 256} : NormPlan{8, 4, 256, 256};
+}
+
+// the backward's workgroups: each has a run of rows of one gate group
 void norm_blocks(const mvr_norm_params *p, int64_t &per_group, int64_t &rows_each, int64_t &blocks) {
+  const NormPlan plan = norm_plan(p->dim);
   const int64_t groups = p->gate_groups ? p->gate_groups : 1, rows = p->rows / groups;
-  const int64_t least = p->dim > 1024 ? 2 : 8;   // rows of a workgroup: below, the partial sums would weigh more than the rows
-  per_group = (1024 + groups - 1) / groups;
+  const int64_t least = plan.waves > 1 ? 2 : 8;   // rows of a workgroup: below, the partial sums would weigh more than the rows
+  per_group = (plan.backward + groups - 1) / groups;
   if (per_group > (rows + least - 1) / least) per_group = (rows + least - 1) / least;
   rows_each = (rows + per_group - 1) / per_group;
   per_group = (rows + rows_each - 1) / rows_each;
@@ -511,26 +587,34 @@ void norm_blocks(const mvr_norm_params *p, int64_t &per_group, int64_t &rows_eac
 
 template <typename TR, typename TB>
 int launch_norm(const NormArgs &a, hipStream_t st) {
-  const bool wide = a.D > 2048;
-  int64_t blocks = wide ? a.rows : (a.rows + 3) / 4;
-  if (blocks > 2048) blocks = 2048;
-  const dim3 g((unsigned)blocks), b(kBlock);
-  if (a.D <= 512) hipLaunchKernelGGL((k_add_norm<TR, TB, 1, 1>), g, b, 0, st, a);
-  else if (a.D <= 1024) hipLaunchKernelGGL((k_add_norm<TR, TB, 1, 2>), g, b, 0, st, a);
-  else if (a.D <= 2048) hipLaunchKernelGGL((k_add_norm<TR, TB, 1, 4>), g, b, 0, st, a);
-  else if (a.D <= 4096) hipLaunchKernelGGL((k_add_norm<TR, TB, 4, 2>), g, b, 0, st, a);
-  else hipLaunchKernelGGL((k_add_norm<TR, TB, 4, 4>), g, b, 0, st, a);
+  const NormPlan plan = norm_plan(a.D);
+  const int64_t blocks = plan.waves > 1 ? a.rows : (a.rows + 3) / 4;
+  const dim3 g((unsigned)(blocks < plan.forward ? blocks : plan.forward)), b(plan.waves > 1 ? 64 * plan.waves : kBlock);
+  switch (plan.waves * 10 + plan.vectors) {
+    case 11: hipLaunchKernelGGL((k_add_norm<TR, TB, 1, 1>), g, b, 0, st, a); break;
+    case 12: hipLaunchKernelGGL((k_add_norm<TR, TB, 1, 2>), g, b, 0, st, a); break;
+    case 13: hipLaunchKernelGGL((k_add_norm<TR, TB, 1, 3>), g, b, 0, st, a); break;
+    case 41: hipLaunchKernelGGL((k_add_norm<TR, TB, 4, 1>), g, b, 0, st, a); break;
+    case 42: hipLaunchKernelGGL((k_add_norm<TR, TB, 4, 2>), g, b, 0, st, a); break;
+    case 82: hipLaunchKernelGGL((k_add_norm<TR, TB, 8, 2>), g, b, 0, st, a); break;
+    default: hipLaunchKernelGGL((k_add_norm<TR, TB, 8, 4>), g, b, 0, st, a);
+  }
   return launched("k_add_norm");
 }
 
 template <typename TR, typename TB>
 int launch_norm_backward(const NormArgs &a, int64_t blocks, hipStream_t st) {
-  const dim3 g((unsigned)blocks), b(kBlock);
-  if (a.D <= 512) hipLaunchKernelGGL((k_add_norm_backward<TR, TB, 1, 1>), g, b, 0, st, a);
-  else if (a.D <= 1024) hipLaunchKernelGGL((k_add_norm_backward<TR, TB, 1, 2>), g, b, 0, st, a);
-  else if (a.D <= 2048) hipLaunchKernelGGL((k_add_norm_backward<TR, TB, 4, 1>), g, b, 0, st, a);
-  else if (a.D <= 4096) hipLaunchKernelGGL((k_add_norm_backward<TR, TB, 4, 2>), g, b, 0, st, a);
-  else hipLaunchKernelGGL((k_add_norm_backward<TR, TB, 4, 4>), g, b, 0, st, a);
+  const NormPlan plan = norm_plan(a.D);
+  const dim3 g((unsigned)blocks), b(plan.waves > 1 ? 64 * plan.waves : kBlock);
+  switch (plan.waves * 10 + plan.vectors) {
+    case 11: hipLaunchKernelGGL((k_add_norm_backward<TR, TB, 1, 1>), g, b, 0, st, a); break;
+    case 12: hipLaunchKernelGGL((k_add_norm_backward<TR, TB, 1, 2>), g, b, 0, st, a); break;
+    case 13: hipLaunchKernelGGL((k_add_norm_backward<TR, TB, 1, 3>), g, b, 0, st, a); break;
+    case 41: hipLaunchKernelGGL((k_add_norm_backward<TR, TB, 4, 1>), g, b, 0, st, a); break;
+    case 42: hipLaunchKernelGGL((k_add_norm_backward<TR, TB, 4, 2>), g, b, 0, st, a); break;
+    case 82: hipLaunchKernelGGL((k_add_norm_backward<TR, TB, 8, 2>), g, b, 0, st, a); break;
+    default: hipLaunchKernelGGL((k_add_norm_backward<TR, TB, 8, 4>), g, b, 0, st, a);
+  }
   return launched("k_add_norm_backward");
 }
 
@@ -607,7 +691,7 @@ extern "C" int mvr_add_norm_tokens_backward(const mvr_norm_params *params, const
   a.blocks_per_group = (int32_t)per, a.block_rows = each;
   if (int rc = MVR_NORM_TYPES(launch_norm_backward, params, a, blocks, (hipStream_t)stream)) return rc;
   if (!columns) return MVR_OK;
-  const dim3 g((unsigned)((params->dim + 63) / 64), 3 + (grad_gate ? (unsigned)params->gate_groups : 0));
+  const dim3 g((unsigned)((params->dim + kColumns - 1) / kColumns), 3 + (grad_gate ? (unsigned)params->gate_groups : 0));
   hipLaunchKernelGGL(k_norm_columns, g, dim3(1024), 0, (hipStream_t)stream, a.partial, params->dim, (int32_t)blocks, (int32_t)per,
                      params->param_type, grad_weight, grad_bias, grad_post_weight, grad_gate);
   return launched("k_norm_columns");
