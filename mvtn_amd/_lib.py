@@ -226,6 +226,25 @@ def torch_op():
     return _TORCH_OP
 
 
+_TOKEN_OP = None
+
+
+def token_op():
+    """`torch.ops.mvr_tokens` — the operators on view tokens with C++ autograd nodes (csrc/mvr_token_op.cpp over the C ABI); the only way
+    to them from Python: raises where it is not built and cannot be."""
+    global _TOKEN_OP
+    if _TOKEN_OP is None:
+        import torch
+        lib = load()
+        torch.ops.load_library(_build.build_torch_op(path=_build.TOKEN_OP_PATH))
+        torch.ops.mvr_tokens.init([ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in
+                                   ("mvr_rotate_tokens_forward", "mvr_rotate_tokens_backward", "mvr_attend_tokens_workspace_bytes", "mvr_attend_tokens_forward",
+                                    "mvr_attend_tokens_backward", "mvr_add_norm_tokens_workspace_bytes", "mvr_add_norm_tokens_forward",
+                                    "mvr_add_norm_tokens_backward", "mvr_last_error")])
+        _TOKEN_OP = torch.ops.mvr_tokens
+    return _TOKEN_OP
+
+
 def check(rc, what=""):
     if rc != MVR_OK:
         msg = load().mvr_last_error()

@@ -14,6 +14,7 @@ CSRC = os.path.join(_HERE, "csrc")
 LIB_PATH = os.path.join(_HERE, "libmvr_hip.so")
 HOSTMATH_PATH = os.path.join(_HERE, "libmvr_hostmath.so")
 TORCH_OP_PATH = os.path.join(_HERE, "_mvr_torch_op.so")
+TOKEN_OP_PATH = os.path.join(_HERE, "_mvr_token_op.so")
 
 HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
                # coverage / depth arithmetic must be the exact IEEE sequence written in mvr_math.h
@@ -154,59 +155,60 @@ def build_hostmath(force=False):
     return HOSTMATH_PATH
 
 
-def _torch_op_sources():
-    return [os.path.join(CSRC, "mvr_torch_op.cpp"), os.path.join(os.path.dirname(_HERE), "include", "mvr.h")]
+def _torch_op_sources(path=TORCH_OP_PATH):
+    return [os.path.join(CSRC, "mvr_torch_op.cpp" if path == TORCH_OP_PATH else "mvr_token_op.cpp"), os.path.join(os.path.dirname(_HERE), "include", "mvr.h")]
 
 
-def torch_op_hash():
-    """Content hash of the torch operator's sources + the torch build it is compiled against (its C++ ABI is torch's)."""
+def torch_op_hash(path=TORCH_OP_PATH):
+    """Content hash of a torch operator's sources + the torch build it is compiled against (its C++ ABI is torch's)."""
     import torch
     # (the version string alone does not pin the C++ ABI: a rebuild of the same version with another libstdc++ ABI or from
     # another commit would otherwise reuse a stale operator)
-    return _src_hash(_torch_op_sources(), ["torch-" + torch.__version__, "cxx11abi-%s" % int(bool(torch._C._GLIBCXX_USE_CXX11_ABI)),
-                                           "git-%s" % getattr(torch.version, "git_version", ""), "hip-%s" % getattr(torch.version, "hip", "")])
+    return _src_hash(_torch_op_sources(path), ["torch-" + torch.__version__, "cxx11abi-%s" % int(bool(torch._C._GLIBCXX_USE_CXX11_ABI)),
+                                               "git-%s" % getattr(torch.version, "git_version", ""), "hip-%s" % getattr(torch.version, "hip", "")])
 
 
-def torch_op_is_current():
+def torch_op_is_current(path=TORCH_OP_PATH):
     try:
-        with open(_hash_path(TORCH_OP_PATH)) as f:
-            return os.path.exists(TORCH_OP_PATH) and f.read().strip() == torch_op_hash()
+        with open(_hash_path(path)) as f:
+            return os.path.exists(path) and f.read().strip() == torch_op_hash(path)
     except OSError:
         return False
 
 
-def build_torch_op(force=False):
+def build_torch_op(force=False, path=TORCH_OP_PATH):
     """g++ -> mvtn_amd/_mvr_torch_op.so: host-side plumbing (csrc/mvr_torch_op.cpp: the mesh step as one torch operator with a
-    C++ autograd node).  No kernels, no link against libmvr_hip.so (the entry points are handed over as addresses); links
-    against the torch of this interpreter.  Same lock / rename discipline as build_hip."""
-    if not force and torch_op_is_current():
-        return TORCH_OP_PATH
+    C++ autograd node), or mvtn_amd/_mvr_token_op.so (csrc/mvr_token_op.cpp: the operators on view tokens).  No kernels, no link
+    against libmvr_hip.so (the entry points are handed over as addresses); links against the torch of this interpreter.  Same
+    lock / rename discipline as build_hip."""
+    if not force and torch_op_is_current(path):
+        return path
     from torch.utils import cpp_extension as ce
     import torch
-    with open(TORCH_OP_PATH + ".lock", "w") as lock:
+    with open(path + ".lock", "w") as lock:
         fcntl.flock(lock, fcntl.LOCK_EX)
         try:
-            if not force and torch_op_is_current():
-                return TORCH_OP_PATH
-            tmp = "%s.tmp.%d" % (TORCH_OP_PATH, os.getpid())
+            if not force and torch_op_is_current(path):
+                return path
+            tmp = "%s.tmp.%d" % (path, os.getpid())
             cmd = (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)] +
-                   ["-I" + d for d in ce.include_paths()] + [_torch_op_sources()[0], "-o", tmp] +
+                   ["-I" + d for d in ce.include_paths()] + [_torch_op_sources(path)[0], "-o", tmp] +
                    ["-L" + d for d in ce.library_paths()] + ["-ltorch", "-ltorch_cpu", "-lc10"])
             try:
                 r = subprocess.run(cmd, capture_output=True, text=True)
                 if r.returncode != 0:
                     raise RuntimeError("g++ failed:\n%s\n%s" % (" ".join(cmd), r.stderr[-4000:]))
-                os.replace(tmp, TORCH_OP_PATH)
+                os.replace(tmp, path)
             finally:
                 if os.path.exists(tmp):
                     os.remove(tmp)
-            htmp = "%s.tmp.%d" % (_hash_path(TORCH_OP_PATH), os.getpid())
+            htmp = "%s.tmp.%d" % (_hash_path(path), os.getpid())
             with open(htmp, "w") as f:
-                f.write(torch_op_hash() + "\n")
-            os.replace(htmp, _hash_path(TORCH_OP_PATH))
+                f.write(torch_op_hash(path) + "\n")
+            os.replace(htmp, _hash_path(path))
         finally:
             fcntl.flock(lock, fcntl.LOCK_UN)
-    return TORCH_OP_PATH
+    return path
 
 
 if __name__ == "__main__":

@@ -395,3 +395,28 @@ def test_attention_matches_the_definition(dtype, B, Lq, Lk, H, E, D, groups, dro
     assert all(torch.equal(a, b) for a, b in zip(again, got[1:]))   # bit-reproducible
     with torch.no_grad():
         assert torch.equal(tokens.attend_tokens(*leaves, keep=keep), got[0])
+
+
+def test_gradients_cannot_be_differentiated_again():
+    """create_graph gives the gradients; a second differentiation fails where it is asked for, and not silently."""
+    g = _gen(12)
+    x = _randn(g, 1, 4, 2, 8).requires_grad_()
+    pos = _randn(g, 4, 1).requires_grad_()
+    h = _randn(g, 1, 4, 2, 8, dtype=torch.bfloat16).requires_grad_()
+    rotary = tokens.TokenRotary((4,))
+    for out, leaf in ((rotary(x, pos), x), (tokens.attend_tokens(h, h, h), h), (tokens.add_norm_tokens(x, x, _randn(g, 8))[1], x)):
+        up = torch.ones_like(out).requires_grad_()
+        first, = torch.autograd.grad(out, leaf, up, create_graph=True)
+        assert torch.isfinite(first).all()
+        with pytest.raises(RuntimeError, match="differentiated"):
+            first.float().sum().backward()
+
+
+def test_saved_tensors_that_were_written_over_are_noticed():
+    g = _gen(13)
+    x, w = _randn(g, 2, 4, 8).requires_grad_(), _randn(g, 8)
+    y, z = tokens.add_norm_tokens(x, x, w)
+    with torch.no_grad():
+        y.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.sum().backward()
