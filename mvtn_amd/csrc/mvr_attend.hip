@@ -37,6 +37,10 @@ template <> struct Vec<f16> { typedef f16x8 type; };
 __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mfma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
 struct AttArgs {
   const void *q, *k, *v, *o, *go;
   const uint8_t *keep;
@@ -49,8 +53,11 @@ struct AttArgs {
   int32_t groups, per;           // keep: (B, groups), `per` keys each
   int32_t rows;                  // G * Lq
   int32_t tiles, splits, split_tiles, col_tiles;
+  int32_t wide;                  // two columns of 32 queries a wave
+  int32_t whole;                 // D a multiple of 8 and a tile's rows within 32-bit offsets: tiles are loaded in whole chunks
   int64_t work;                  // workgroups with something to do
   float c, scale;                // scale log2(e)
+  double per_inverse;            // 1 / per
 };
 
 // Workgroups are dealt to the 8 XCDs round robin: item = a contiguous run of the work per XCD, so that the workgroups which read one
@@ -75,46 +82,143 @@ __device__ __forceinline__ u32x4 load16(const T *p, int left) {
   return r;
 }
 
-// A tile of kTile rows on its way from memory to LDS; `row` gives a row's address, or null for a row of zeros
-template <typename T, int DP>
+// How a tile lies in LDS: rows of 4, 8 or 16 chunks of 16 bytes, chunk c of row r at c ^ swizzle(r), so that no way of reading it meets a bank
+// twice: 16 rows at one chunk (row_frag), 4 rows at 4 chunks or 8 rows at 2 (col_frag) each fall on 16 different bank groups of the 64 banks.
+template <int DP>
+struct Layout {
+  static constexpr int kChunks = DP <= 32 ? 4 : DP <= 64 ? 8 : 16, kPitch = 8 * kChunks, kSize = kTile * kPitch;
+  static __device__ __forceinline__ int swizzle(int r) {
+    const int low = (r >> 2 & 1) << 1 | (r >> 3 & 1);
+    return DP <= 32 ? low : DP <= 64 ? (r >> 1 & 1) << 2 | low : (r & 3) << 2 | low;
+  }
+};
+
+// A tile of kTile rows on its way from memory to LDS
+template <typename T, int DP, int THREADS = kBlock>
 struct Stage {
-  static constexpr int kChunks = kTile * DP / 8 / kBlock, kPitch = DP + 8;
+  static constexpr int kPerRow = DP / 8, kChunks = (kTile * kPerRow + THREADS - 1) / THREADS;
+  static constexpr bool kEven = THREADS % kPerRow == 0;   // a thread's chunks lie in one column, THREADS / kPerRow rows apart
+  static constexpr bool kPart = kTile * kPerRow % THREADS != 0;   // the last chunk is not for every thread
   u32x4 r[kChunks];
+  __device__ __forceinline__ Stage() {
+#pragma unroll
+    for (int k = 0; k < kChunks; ++k) r[k] = u32x4{0, 0, 0, 0};
+  }
+  // D a multiple of 8, rows `stride` elements apart, the last of them again for what lies behind it: one way for whole tiles and ends, as loads
+  // on two ways into the same registers are copied, and waited for, where the ways meet
+  __device__ __forceinline__ void load(const T *base, unsigned stride, int D, unsigned last) {
+    if constexpr (kEven && !kPart) {
+      const unsigned i = threadIdx.x / kPerRow, c = threadIdx.x % kPerRow * 8;
+      if (c < (unsigned)D) {   // (chunks behind a head stay the zeros they are)
+        unsigned at = i * stride + c;
+        const unsigned end = last * stride + c;
+        asm volatile("" : "+v"(at));   // (one address is kept through the loop, not one per chunk)
+#pragma unroll
+        for (int k = 0; k < kChunks; ++k) {
+          const unsigned x = at + k * (THREADS / kPerRow) * stride;
+          __builtin_memcpy(&r[k], base + (x < end ? x : end), 16);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kChunks; ++k) {
+        const unsigned e = threadIdx.x + k * THREADS, i = e / kPerRow, c = e % kPerRow * 8;
+        if (c < (unsigned)D && (!kPart || i < kTile)) __builtin_memcpy(&r[k], base + (i < last ? i : last) * stride + c, 16);
+      }
+    }
+  }
+  // `row` gives a row's address, or null for a row of zeros
   template <typename Row>
-  __device__ __forceinline__ void load(int D, Row row) {
+  __device__ __forceinline__ void load_rows(int D, Row row) {
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));   // (its addresses are not to be kept in registers all through the loop)
 #pragma unroll
     for (int k = 0; k < kChunks; ++k) {
-      const int e = threadIdx.x + k * kBlock, i = e / (DP / 8), c = e % (DP / 8) * 8;
-      const T *p = row(i);
+      const int e = tid + k * THREADS, i = e / kPerRow, c = e % kPerRow * 8;
+      const T *p = kPart && i >= kTile ? nullptr : row(i);
       r[k] = load16(p + c, p ? D - c : 0);
     }
   }
-  __device__ __forceinline__ void store(T *lds) const {
+  // rows whose bit is not set become zeros
+  __device__ __forceinline__ void store(T *lds, unsigned long long rows) const {
+    const int i0 = threadIdx.x / kPerRow, at0 = i0 * Layout<DP>::kPitch + (threadIdx.x % kPerRow ^ Layout<DP>::swizzle(i0)) * 8;
 #pragma unroll
     for (int k = 0; k < kChunks; ++k) {
-      const int e = threadIdx.x + k * kBlock, i = e / (DP / 8), c = e % (DP / 8) * 8;
-      *reinterpret_cast<u32x4 *>(lds + i * kPitch + c) = r[k];
+      const int e = threadIdx.x + k * THREADS, i = e / kPerRow;
+      u32x4 x = r[k];
+      if (rows != ~0ull && !(rows >> (i & 63) & 1)) x = u32x4{0, 0, 0, 0};
+      // (whole multiples of 16 rows apart the swizzle is the same)
+      const int at = kEven && THREADS / kPerRow % 16 == 0 ? at0 + k * (THREADS / kPerRow) * Layout<DP>::kPitch
+                                                          : i * Layout<DP>::kPitch + (e % kPerRow ^ Layout<DP>::swizzle(i)) * 8;
+      if (!kPart || i < kTile) *reinterpret_cast<u32x4 *>(lds + at) = x;
     }
   }
 };
 
-// operand with the tile's rows 32 t + (lane % 32) as its rows, d = 16 s + 8 (lane / 32) + 0..7 as its depth
+// Where this lane reads a tile.  A swizzled address is a base with bits flipped, so three bases give all of them; `at` makes fresh copies for one
+// step: addresses that follow from them are not kept in registers all through a loop.
+typedef __attribute__((address_space(3))) char lds_char;
+template <int DP>
+struct Reader {
+  static constexpr int kRow = 2 * Layout<DP>::kPitch, kBytes = kTile * kRow;   // of 16-bit elements
+  unsigned row, col, col8;
+  // 32 x 32 x 16: row_frag has the tile's rows 32 t + (lane % 32) as its rows, d = 16 s + 8 (lane / 32) + 0..7 as its depth;
+  // col_frag d = 32 db + (lane % 32) as its rows, the tile's rows 16 s + 4 (lane / 32) + {0..3, 8..11} as its depth
+  static __device__ __forceinline__ Reader wide(const void *lds) {
+    const unsigned lane = threadIdx.x & 63, i = lane & 31, j = 4 * (lane >> 5) + (lane >> 2 & 3), x = (lane >> 4 & 1) * 2 + (lane >> 1 & 1);
+    const unsigned base = (unsigned)(size_t)(lds_char *)lds;
+    Reader r;
+    r.row = base + i * kRow + ((lane >> 5) ^ Layout<DP>::swizzle(i)) * 16;
+    r.col = base + j * kRow + (x ^ Layout<DP>::swizzle(j)) * 16 + 8 * (lane & 1);
+    r.col8 = base + (j + 8) * kRow + (x ^ Layout<DP>::swizzle(j + 8)) * 16 + 8 * (lane & 1);
+    return r;
+  }
+  // 16 x 16 x 32: rows 16 b + (lane % 16), d = 32 s + 8 (lane / 16) + 0..7;  d = 16 db + (lane % 16), rows 32 t + 4 (lane / 16) + {0..3, 16..19}
+  static __device__ __forceinline__ Reader narrow(const void *lds) {
+    const unsigned lane = threadIdx.x & 63, i = lane & 15, j = 4 * (lane >> 4) + (lane >> 2 & 3), base = (unsigned)(size_t)(lds_char *)lds;
+    Reader r;
+    r.row = base + i * kRow + ((lane >> 4) ^ Layout<DP>::swizzle(i)) * 16;
+    r.col = base + j * kRow + ((lane >> 1 & 1) ^ Layout<DP>::swizzle(j)) * 16 + 8 * (lane & 1);
+    r.col8 = 0;
+    return r;
+  }
+  __device__ __forceinline__ Reader at(int buffer) const {   // of the two tiles of a buffer, the first
+    Reader r = {row + buffer * 2 * kBytes, col + buffer * 2 * kBytes, col8 + buffer * 2 * kBytes};
+    asm volatile("" : "+v"(r.row), "+v"(r.col), "+v"(r.col8));
+    return r;
+  }
+  template <typename V>
+  static __device__ __forceinline__ V load(unsigned at) {
+    return *(const __attribute__((address_space(3))) V *)(lds_char *)(size_t)at;
+  }
+  template <typename V>
+  static __device__ __forceinline__ V load_columns(unsigned at, unsigned more) {
+    typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+    union { i16x4 h[2]; V v; } u;
+    u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(lds_char *)(size_t)at);
+    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(lds_char *)(size_t)more);
+    return u.v;
+  }
+};
+// the operands of one sub-tile of 32 rows, of a buffer's first or second tile
 template <typename T, int DP>
-__device__ __forceinline__ typename Vec<T>::type row_frag(const T *lds, int t, int s) {
-  const int lane = threadIdx.x & 63;
-  return *reinterpret_cast<const typename Vec<T>::type *>(lds + (32 * t + (lane & 31)) * (DP + 8) + 16 * s + 8 * (lane >> 5));
+__device__ __forceinline__ void row_frags(const Reader<DP> &r, int which, int t, typename Vec<T>::type (&f)[DP / 16]) {
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) f[s] = Reader<DP>::template load<typename Vec<T>::type>((r.row ^ 32 * s) + which * r.kBytes + 32 * t * r.kRow);
 }
-// operand with d = 32 db + (lane % 32) as its rows, the tile's rows 16 s + 4 (lane / 32) + {0..3, 8..11} as its depth
 template <typename T, int DP>
-__device__ __forceinline__ typename Vec<T>::type col_frag(const T *lds, int s, int db) {
-  typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
-  const int lane = threadIdx.x & 63;
-  const T *p = lds + (16 * s + 4 * (lane >> 5) + ((lane & 15) >> 2)) * (DP + 8) + 32 * db + (lane & 16) + 4 * (lane & 3);
-  union { i16x4 h[2]; typename Vec<T>::type v; } u;
-  u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)p);
-  u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(p + 8 * (DP + 8)));
-  return u.v;
+__device__ __forceinline__ void col_frags(const Reader<DP> &r, int which, int t, typename Vec<T>::type (&f)[2][DP / 32]) {
+#pragma unroll
+  for (int half = 0; half < 2; ++half)
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) {
+      const int off = which * r.kBytes + (32 * t + 16 * half) * r.kRow;
+      f[half][d] = Reader<DP>::template load_columns<typename Vec<T>::type>((r.col ^ 64 * d) + off, (r.col8 ^ 64 * d) + off);
+    }
 }
+// Nothing moves across: operands of the next products are not all read at once (the registers are full)
+__device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
+
 template <typename T>
 __device__ __forceinline__ typename Vec<T>::type to_frag(const f32x16 &x, int half) {
   typename Vec<T>::type v;
@@ -122,66 +226,175 @@ __device__ __forceinline__ typename Vec<T>::type to_frag(const f32x16 &x, int ha
   for (int k = 0; k < 8; ++k) v[k] = (T)x[8 * half + k];
   return v;
 }
-// rows of a tensor straight into operands: this lane's row p (null: zeros)
-template <typename T, int DP>
-__device__ __forceinline__ void load_frags(const T *p, int D, typename Vec<T>::type (&f)[DP / 16]) {
-  const int hi = (threadIdx.x & 63) >> 5;
+// x + the sum of an operand's eight values
+__device__ __forceinline__ float add_frag(bf16x8 p, float x) {
+  typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 one = {(bf16)1.0f, (bf16)1.0f};
+  bf16x2 h[4];
+  __builtin_memcpy(h, &p, 16);
 #pragma unroll
-  for (int s = 0; s < DP / 16; ++s) {
-    const u32x4 r = load16(p + 16 * s + 8 * hi, p ? D - 16 * s - 8 * hi : 0);
-    __builtin_memcpy(&f[s], &r, 16);
+  for (int k = 0; k < 4; ++k) x = __builtin_amdgcn_fdot2_f32_bf16(h[k], one, x, false);
+  return x;
+}
+__device__ __forceinline__ float add_frag(f16x8 p, float x) {
+  typedef f16 f16x2 __attribute__((ext_vector_type(2)));
+  const f16x2 one = {(f16)1.0f, (f16)1.0f};
+  f16x2 h[4];
+  __builtin_memcpy(h, &p, 16);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) x = __builtin_amdgcn_fdot2(h[k], one, x, false);
+  return x;
+}
+// Waits for every load issued so far.  Called in front of a loop that keeps loads in flight: a register loaded before the loop would otherwise
+// be waited for inside it, and the wait for it is a wait for everything.
+__device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0F70); }   // vmcnt(0)
+
+// A row of a tensor straight into operands.  (A column without a query reads the first one's row: nothing of it is stored.)
+template <typename T, int DP>
+__device__ __forceinline__ void load_frags(const T *p, const AttArgs &a, typename Vec<T>::type (&f)[DP / 16]) {
+  const int hi = (threadIdx.x & 63) >> 5;
+  if (a.D == DP) {
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) __builtin_memcpy(&f[s], p + 16 * s + 8 * hi, 16);
+  } else {
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) {
+      const u32x4 r = load16(p + 16 * s + 8 * hi, a.D - 16 * s - 8 * hi);
+      __builtin_memcpy(&f[s], &r, 16);
+    }
   }
+}
+
+// key / per: the quotient in 64 bits is off by one at most, and put right
+__device__ __forceinline__ int group_of(const AttArgs &a, int key) {
+  int g = (int)(key * a.per_inverse);
+  const int rest = key - g * a.per;
+  return rest < 0 ? g - 1 : rest >= a.per ? g + 1 : g;
 }
 
 // which of a tile's keys are there, one bit each
 __device__ __forceinline__ unsigned long long tile_keys(const AttArgs &a, int b, int tile) {
   const int key = tile * kTile + (threadIdx.x & 63);
   bool on = key < a.Lk;
-  if (a.keep && on) on = a.keep[(int64_t)b * a.groups + key / a.per] != 0;
+  if (a.keep && on) on = a.keep[(int64_t)b * a.groups + group_of(a, key)] != 0;
   return __ballot(on);
-}
-
-// Walks the tiles [first, last) of one object that hold a kept key; step(tile, keys) is called by all waves alike
-template <typename Load, typename Store, typename Step>
-__device__ __forceinline__ void walk_tiles(const AttArgs &a, int b, int first, int last, Load load, Store store, Step step) {
-  __shared__ unsigned long long masks[64];
-  const int wave = threadIdx.x >> 6;
-  for (int c0 = first; c0 < last; c0 += 64) {
-    const int n = last - c0 < 64 ? last - c0 : 64;
-    lds_barrier();   // the previous chunk's masks and tiles have been read
-    for (int i = wave; i < n; i += kWaves) {
-      const unsigned long long m = tile_keys(a, b, c0 + i);
-      if ((threadIdx.x & 63) == 0) masks[i] = m;
-    }
-    lds_barrier();
-    int i = 0;
-    while (i < n && !masks[i]) ++i;
-    unsigned long long m = i < n ? masks[i] : 0;
-    if (i < n) load(c0 + i, m);
-    while (i < n) {
-      lds_barrier();
-      store();
-      lds_barrier();
-      int next = i + 1;
-      while (next < n && !masks[next]) ++next;
-      const unsigned long long mn = next < n ? masks[next] : 0;
-      if (next < n) load(c0 + next, mn);
-      step(c0 + i, m);
-      i = next, m = mn;
-    }
-  }
 }
 
 __device__ __forceinline__ unsigned long long uniform(unsigned long long m) {
   return (unsigned long long)__builtin_amdgcn_readfirstlane((int)(m >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)m);
 }
 
+// Walks the tiles [first, last) of one object that hold a kept key, two buffers in turn.  The work on a tile comes in two halves, step(buffer, keys, 0)
+// and (.., 1); beside the first the next tile's k is on its way, beside the second its v (one set of registers for both), each stored into
+// the other buffer afterwards.  both(tile, keys) brings a first tile into buffer 0.  All waves make the same calls.
+template <typename Both, typename Load, typename Store, typename Step>
+__device__ __forceinline__ void walk_tiles(const AttArgs &a, int b, int first, int last, Both both, Load load, Store store, Step step) {
+  __shared__ unsigned long long masks[64];
+  const int wave = threadIdx.x >> 6;
+  for (int c0 = first; c0 < last; c0 += 64) {
+    const int n = last - c0 < 64 ? last - c0 : 64;
+    for (int i = wave; i < n; i += kWaves) {
+      const unsigned long long m = tile_keys(a, b, c0 + i);
+      if ((threadIdx.x & 63) == 0) masks[i] = m;
+    }
+    lds_barrier();
+    int i = 0, buffer = 0;
+    while (i < n && !masks[i]) ++i;
+    unsigned long long m = i < n ? uniform(masks[i]) : 0;
+    if (i < n) both(c0 + i, m);
+    loads_done();
+    lds_barrier();
+    while (i < n) {
+      int next = i + 1;
+      while (next < n && !masks[next]) ++next;
+      const unsigned long long mn = next < n ? uniform(masks[next]) : 0;
+      if (next < n) load(0, c0 + next);
+      step(buffer, m, 0);
+      if (next < n) {
+        store(0, buffer ^ 1, mn);
+        load(1, c0 + next);
+      }
+      step(buffer, m, 1);
+      buffer ^= 1;
+      if (next < n) store(1, buffer, mn);
+      lds_barrier();
+      i = next, m = mn;
+    }
+  }
+}
+
+// what walk_tiles is told for tiles of k and v
+#define MVR_ATT_KV                                                                                                      \
+  [&](int tile, unsigned long long m) {                                                                                 \
+    Stage<T, DP> more;                                                                                                  \
+    load_tile<WHOLE>(staged, kb, a.ks[1], tile, a);                                                                            \
+    load_tile<WHOLE>(more, vb, a.vs[1], tile, a);                                                                              \
+    staged.store(tiles[0], m), more.store(tiles[0] + kSize, m);                                                         \
+  },                                                                                                                    \
+      [&](int which, int tile) { load_tile<WHOLE>(staged, which ? vb : kb, which ? a.vs[1] : a.ks[1], tile, a); },             \
+      [&](int which, int buffer, unsigned long long m) { staged.store(tiles[buffer] + which * kSize, m); }
+
+template <bool WHOLE, typename T, int DP>
+__device__ __forceinline__ void load_tile(Stage<T, DP> &staged, const T *base, int64_t stride, int tile, const AttArgs &a) {
+  const int at = tile * kTile, left = a.Lk - at;
+  base += at * stride;
+  if constexpr (WHOLE) staged.load(base, (unsigned)stride, a.D, left < kTile ? left - 1 : kTile - 1);
+  else staged.load_rows(a.D, [&](int r) { return r < left ? base + r * stride : nullptr; });
+}
+
 // ---- forward -----------------------------------------------------------------------------------------------------
 
-template <typename T, int DP, bool SPLIT>
+// A lane's column: the query (of one of the group's heads) that it works for
+struct Column {
+  int64_t row;
+  int g, i;
+  bool live;
+};
+__device__ __forceinline__ Column column_of(const AttArgs &a, int ct, int n, int per_wave) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  Column c;
+  c.row = ((int64_t)ct * kWaves + wave) * per_wave + 32 * n + (lane & 31);
+  c.live = c.row < a.rows;
+  c.g = c.live ? (int)((unsigned)c.row / (unsigned)a.Lq) : 0;
+  c.i = c.live ? (int)c.row - c.g * a.Lq : 0;
+  return c;
+}
+// a column's 32 db values, four by four in the order of the matrix instruction's result
+template <typename U, int DP>
+__device__ __forceinline__ void store_column(U *p, int D, const f32x16 (&x)[DP / 32], float f) {
+  const int hi = (threadIdx.x & 63) >> 5;
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int at = 32 * d + 8 * r + 4 * hi;
+      const float v[4] = {x[d][4 * r] * f, x[d][4 * r + 1] * f, x[d][4 * r + 2] * f, x[d][4 * r + 3] * f};
+      store_n<4>(p + at, D == DP ? 4 : D - at, v);
+    }
+}
+// the scores of keys that are not there, replaced: a register's 32 + 32 lanes hold two keys, so their bits make its lane mask on the scalar unit
+__device__ __forceinline__ void mask_scores(f32x16 &s, unsigned long long m, int t, float by) {
+  const unsigned bits = (unsigned)(m >> (32 * t));
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int at = 8 * (r / 4) + r % 4;
+    const unsigned lo = bits >> at & 1 ? ~0u : 0u, hi = bits >> (at + 4) & 1 ? ~0u : 0u;
+    s[r] = __builtin_amdgcn_inverse_ballot_w64((unsigned long long)hi << 32 | lo) ? s[r] : by;
+  }
+}
+
+// The running maximum only has to keep exponentials in range: it follows the scores when one exceeds it by more than kSlack (powers of two),
+// and only then are sum and output rescaled.  Probabilities then reach 2^8, far from any type's limit, and their rounding is relative.
+// (Following every new maximum, one of a wave's 64 columns has one in four tiles of five, at 68 multiplications each.)
+constexpr float kSlack = 8.0f;
+
+// NS columns of 32 queries a wave: with two, every operand read from LDS serves two products, and one's exponentials run beside the other's
+// products
+template <typename T, int DP, int NS, bool SPLIT, bool WHOLE>
 __global__ __launch_bounds__(kBlock, 2) void k_attend(AttArgs a) {
   typedef typename Vec<T>::type V8;
-  __shared__ __attribute__((aligned(16))) T kt[kTile * (DP + 8)], vt[kTile * (DP + 8)];
+  constexpr int kSize = Layout<DP>::kSize;
+  __shared__ __attribute__((aligned(256))) T tiles[2][2 * kSize];   // two buffers of a tile of k and a tile of v
   int64_t item = work_item(a.work);
   if (item >= a.work) return;
   const int split = SPLIT ? (int)(item % a.splits) : 0;
@@ -189,100 +402,100 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend(AttArgs a) {
   const int ct = (int)(item % a.col_tiles);
   const int64_t be = item / a.col_tiles;
   const int b = (int)(be / a.E), e = (int)(be - (int64_t)b * a.E);
-  const int lane = threadIdx.x & 63, hi = lane >> 5, wave = threadIdx.x >> 6;
-  const int64_t row = (int64_t)ct * (32 * kWaves) + wave * 32 + (lane & 31);
-  const bool live = row < a.rows;
-  const int g = live ? (int)(row / a.Lq) : 0, i = live ? (int)(row - (int64_t)g * a.Lq) : 0, h = e * a.G + g;
-  V8 q[DP / 16];
-  load_frags<T, DP>(live ? (const T *)a.q + b * a.qs[0] + i * a.qs[1] + h * a.qs[2] : nullptr, a.D, q);
-  const T *kb = (const T *)a.k + b * a.ks[0] + e * a.ks[2], *vb = (const T *)a.v + b * a.vs[0] + e * a.vs[2];
-  f32x16 o[DP / 32];
+  V8 q[NS][DP / 16];
+  f32x16 o[NS][DP / 32];
+  float top[NS], sum[NS];   // of this lane's column; the sum over the rows this lane holds
 #pragma unroll
-  for (int d = 0; d < DP / 32; ++d) o[d] = 0.0f;
-  float top = -INFINITY, sum = 0.0f;   // of this lane's column; the sum over the rows this lane holds
-  Stage<T, DP> ks, vs;
+  for (int n = 0; n < NS; ++n) {
+    const Column c = column_of(a, ct, n, 32 * NS);
+    load_frags<T, DP>((const T *)a.q + b * a.qs[0] + c.i * a.qs[1] + (e * a.G + c.g) * a.qs[2], a, q[n]);
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) o[n][d] = 0.0f;
+    top[n] = -INFINITY, sum[n] = 0.0f;
+  }
+  const T *kb = (const T *)a.k + b * a.ks[0] + e * a.ks[2], *vb = (const T *)a.v + b * a.vs[0] + e * a.vs[2];
+  Stage<T, DP> staged;
+  const Reader<DP> reader = Reader<DP>::wide(tiles);
   const int first = SPLIT ? split * a.split_tiles : 0, last = SPLIT && first + a.split_tiles < a.tiles ? first + a.split_tiles : a.tiles;
+  f32x16 s[NS][2];
   walk_tiles(
       a, b, first, last,
-      [&](int tile, unsigned long long m) {
-        const int64_t at = (int64_t)tile * kTile;
-        ks.load(a.D, [&](int r) { return m >> r & 1 ? kb + (at + r) * a.ks[1] : nullptr; });
-        vs.load(a.D, [&](int r) { return m >> r & 1 ? vb + (at + r) * a.vs[1] : nullptr; });
-      },
-      [&]() { ks.store(kt), vs.store(vt); },
-      [&](int, unsigned long long m) {
-        m = uniform(m);
-        f32x16 s[2];
+      MVR_ATT_KV,
+      [&](int buffer, unsigned long long m, int half) {
+        const Reader<DP> r = reader.at(buffer);
+        if (half == 1) {   // probabilities and their product with v
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            V8 v[2][DP / 32], p[NS][2];
+            col_frags<T, DP>(r, 1, t, v);
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+              const float off = top[n] == -INFINITY ? 0.0f : top[n];
+#pragma unroll
+              for (int r = 0; r < 16; ++r) s[n][t][r] = __builtin_amdgcn_exp2f(fmaf(s[n][t][r], a.c, -off));
+              p[n][0] = to_frag<T>(s[n][t], 0), p[n][1] = to_frag<T>(s[n][t], 1);
+              sum[n] = add_frag(p[n][1], add_frag(p[n][0], sum[n]));   // (of the probabilities as they enter the product)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d) o[n][d] = mfma(v[h][d], p[n][h], o[n][d]);
+            }
+          }
+          return;
+        }
+        // scores, running maximum
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          s[t] = 0.0f;
+          V8 k[DP / 16];
+          row_frags<T, DP>(r, 0, t, k);
 #pragma unroll
-          for (int d = 0; d < DP / 16; ++d) s[t] = mfma(row_frag<T, DP>(kt, t, d), q[d], s[t]);
+          for (int n = 0; n < NS; ++n) {
+            s[n][t] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d) s[n][t] = mfma(k[d], q[n][d], s[n][t]);
+          }
         }
         if (m != ~0ull) {
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const unsigned bits = (unsigned)(m >> (32 * t)) >> (4 * hi);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[t][r] = bits >> (8 * (r / 4) + r % 4) & 1 ? s[t][r] : -INFINITY;
-          }
+          for (int n = 0; n < NS; ++n) mask_scores(s[n][0], m, 0, -INFINITY), mask_scores(s[n][1], m, 1, -INFINITY);
         }
-        float mx = s[0][0];
+        float now[NS];
+        bool up = false;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int n = 0; n < NS; ++n) {
+          float mx = fmaxf(s[n][0][0], s[n][1][0]);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[t][r]);
-        mx = fmaxf(mx, other_half(mx));
-        const float now = fmaxf(top, mx * a.c);
-        if (__any(now > top)) {
-          const float f = __builtin_amdgcn_exp2f(top - (now == -INFINITY ? 0.0f : now));
-          sum *= f;
-#pragma unroll
-          for (int d = 0; d < DP / 32; ++d) o[d] *= f;
-          top = now;
+          for (int r = 1; r < 16; ++r) mx = fmaxf(fmaxf(s[n][0][r], s[n][1][r]), mx);
+          mx = fmaxf(mx, other_half(mx));
+          now[n] = fmaxf(top[n], mx * a.c);
+          up = up || now[n] > top[n] + kSlack;
         }
-        const float off = top == -INFINITY ? 0.0f : top;
+        if (__any(up)) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+          for (int n = 0; n < NS; ++n) {
+            const float f = __builtin_amdgcn_exp2f(top[n] - (now[n] == -INFINITY ? 0.0f : now[n]));
+            sum[n] *= f;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            s[t][r] = __builtin_amdgcn_exp2f(fmaf(s[t][r], a.c, -off));
-            sum += s[t][r];
-          }
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const V8 p = to_frag<T>(s[t], half);
-#pragma unroll
-            for (int d = 0; d < DP / 32; ++d) o[d] = mfma(col_frag<T, DP>(vt, 2 * t + half, d), p, o[d]);
+            for (int d = 0; d < DP / 32; ++d) o[n][d] *= f;
+            top[n] = now[n];
           }
         }
       });
-  sum += other_half(sum);
-  if (!live) return;
-  const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;   // (a NaN stays one)
-  if constexpr (SPLIT) {
-    const int64_t line = (split * (int64_t)a.B * a.E + be) * a.rows + row;
-    float *p = a.part + line * a.D;
+  const int hi = (threadIdx.x & 63) >> 5;
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int at = 32 * d + 8 * r + 4 * hi;
-        const float x[4] = {o[d][4 * r] * inv, o[d][4 * r + 1] * inv, o[d][4 * r + 2] * inv, o[d][4 * r + 3] * inv};
-        store_n<4>(p + at, a.D - at, x);
-      }
-    if (hi == 0) a.part_lse[line] = sum == 0.0f ? -INFINITY : top + __builtin_amdgcn_logf(sum);
-  } else {
-    T *p = (T *)a.out + (((int64_t)b * a.Lq + i) * a.H + h) * a.D;
-#pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int at = 32 * d + 8 * r + 4 * hi;
-        const float x[4] = {o[d][4 * r] * inv, o[d][4 * r + 1] * inv, o[d][4 * r + 2] * inv, o[d][4 * r + 3] * inv};
-        store_n<4>(p + at, a.D - at, x);
-      }
-    if (a.lse && hi == 0) a.lse[be * a.rows + row] = sum == 0.0f ? INFINITY : top + __builtin_amdgcn_logf(sum);
+  for (int n = 0; n < NS; ++n) {
+    const Column c = column_of(a, ct, n, 32 * NS);
+    const float all = sum[n] + other_half(sum[n]);
+    if (!c.live) continue;
+    const float inv = all > 0.0f ? 1.0f / all : all == 0.0f ? 0.0f : all;   // (a NaN stays one)
+    if constexpr (SPLIT) {
+      const int64_t line = (split * (int64_t)a.B * a.E + be) * a.rows + c.row;
+      store_column<float, DP>(a.part + line * a.D, a.D, o[n], inv);
+      if (hi == 0) a.part_lse[line] = all == 0.0f ? -INFINITY : top[n] + __builtin_amdgcn_logf(all);
+    } else {
+      store_column<T, DP>((T *)a.out + (((int64_t)b * a.Lq + c.i) * a.H + e * a.G + c.g) * a.D, a.D, o[n], inv);
+      if (a.lse && hi == 0) a.lse[be * a.rows + c.row] = all == 0.0f ? INFINITY : top[n] + __builtin_amdgcn_logf(all);
+    }
   }
 }
 
@@ -312,10 +525,11 @@ __global__ __launch_bounds__(kBlock) void k_attend_join(AttArgs a) {
 
 // ---- dQ (and delta) ----------------------------------------------------------------------------------------------
 
-template <typename T, int DP, bool SPLIT>
+template <typename T, int DP, int NS, bool SPLIT, bool WHOLE>
 __global__ __launch_bounds__(kBlock, 2) void k_attend_dq(AttArgs a) {
   typedef typename Vec<T>::type V8;
-  __shared__ __attribute__((aligned(16))) T kt[kTile * (DP + 8)], vt[kTile * (DP + 8)];
+  constexpr int kSize = Layout<DP>::kSize;
+  __shared__ __attribute__((aligned(256))) T tiles[2][2 * kSize];   // two buffers of a tile of k and a tile of v
   int64_t item = work_item(a.work);
   if (item >= a.work) return;
   const int split = SPLIT ? (int)(item % a.splits) : 0;
@@ -323,85 +537,81 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dq(AttArgs a) {
   const int ct = (int)(item % a.col_tiles);
   const int64_t be = item / a.col_tiles;
   const int b = (int)(be / a.E), e = (int)(be - (int64_t)b * a.E);
-  const int lane = threadIdx.x & 63, hi = lane >> 5, wave = threadIdx.x >> 6;
-  const int64_t row = (int64_t)ct * (32 * kWaves) + wave * 32 + (lane & 31);
-  const bool live = row < a.rows;
-  const int g = live ? (int)(row / a.Lq) : 0, i = live ? (int)(row - (int64_t)g * a.Lq) : 0, h = e * a.G + g;
-  V8 q[DP / 16], go[DP / 16];
-  load_frags<T, DP>(live ? (const T *)a.q + b * a.qs[0] + i * a.qs[1] + h * a.qs[2] : nullptr, a.D, q);
-  load_frags<T, DP>(live ? (const T *)a.go + b * a.gs[0] + i * a.gs[1] + h * a.gs[2] : nullptr, a.D, go);
-  float delta = 0.0f;
-  {
-    const T *p = live ? (const T *)a.o + (((int64_t)b * a.Lq + i) * a.H + h) * a.D : nullptr;
+  V8 q[NS][DP / 16], go[NS][DP / 16];
+  f32x16 dq[NS][DP / 32];
+  float lse[NS], delta[NS];
+#pragma unroll
+  for (int n = 0; n < NS; ++n) {
+    const Column c = column_of(a, ct, n, 32 * NS);
+    const int h = e * a.G + c.g;
+    load_frags<T, DP>((const T *)a.q + b * a.qs[0] + c.i * a.qs[1] + h * a.qs[2], a, q[n]);
+    load_frags<T, DP>((const T *)a.go + b * a.gs[0] + c.i * a.gs[1] + h * a.gs[2], a, go[n]);
     V8 o[DP / 16];
-    load_frags<T, DP>(p, a.D, o);
+    load_frags<T, DP>((const T *)a.o + (((int64_t)b * a.Lq + c.i) * a.H + h) * a.D, a, o);
+    delta[n] = 0.0f;
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) delta += (float)o[s][k] * (float)go[s][k];
-    delta += other_half(delta);
-  }
-  const float lse = live ? a.lse[be * a.rows + row] : INFINITY;
-  if (live && hi == 0 && split == 0) a.delta[be * a.rows + row] = delta;
-  const T *kb = (const T *)a.k + b * a.ks[0] + e * a.ks[2], *vb = (const T *)a.v + b * a.vs[0] + e * a.vs[2];
-  f32x16 dq[DP / 32];
+      for (int k = 0; k < 8; ++k) delta[n] += (float)o[s][k] * (float)go[n][s][k];
+    delta[n] += other_half(delta[n]);
+    lse[n] = c.live ? a.lse[be * a.rows + c.row] : INFINITY;
+    if (c.live && (threadIdx.x & 32) == 0 && split == 0) a.delta[be * a.rows + c.row] = delta[n];
 #pragma unroll
-  for (int d = 0; d < DP / 32; ++d) dq[d] = 0.0f;
-  Stage<T, DP> ks, vs;
+    for (int d = 0; d < DP / 32; ++d) dq[n][d] = 0.0f;
+  }
+  const T *kb = (const T *)a.k + b * a.ks[0] + e * a.ks[2], *vb = (const T *)a.v + b * a.vs[0] + e * a.vs[2];
+  Stage<T, DP> staged;
+  const Reader<DP> reader = Reader<DP>::wide(tiles);
   const int first = SPLIT ? split * a.split_tiles : 0, last = SPLIT && first + a.split_tiles < a.tiles ? first + a.split_tiles : a.tiles;
   walk_tiles(
       a, b, first, last,
-      [&](int tile, unsigned long long m) {
-        const int64_t at = (int64_t)tile * kTile;
-        ks.load(a.D, [&](int r) { return m >> r & 1 ? kb + (at + r) * a.ks[1] : nullptr; });
-        vs.load(a.D, [&](int r) { return m >> r & 1 ? vb + (at + r) * a.vs[1] : nullptr; });
-      },
-      [&]() { ks.store(kt), vs.store(vt); },
-      [&](int, unsigned long long m) {
-        m = uniform(m);
+      MVR_ATT_KV,
+      [&](int buffer, unsigned long long m, int t) {
+        const Reader<DP> r = reader.at(buffer);
+        V8 f[DP / 16], kc[2][DP / 32];
+        f32x16 s[NS], dp[NS];
+        row_frags<T, DP>(r, 0, t, f);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          f32x16 s = 0.0f, dp = 0.0f;
+        for (int n = 0; n < NS; ++n) {
+          s[n] = 0.0f;
 #pragma unroll
-          for (int d = 0; d < DP / 16; ++d) s = mfma(row_frag<T, DP>(kt, t, d), q[d], s);
-#pragma unroll
-          for (int d = 0; d < DP / 16; ++d) dp = mfma(row_frag<T, DP>(vt, t, d), go[d], dp);
-          const unsigned bits = (unsigned)(m >> (32 * t)) >> (4 * hi);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse));
-            if (m != ~0ull) p = bits >> (8 * (r / 4) + r % 4) & 1 ? p : 0.0f;
-            s[r] = p * (dp[r] - delta);
-          }
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const V8 ds = to_frag<T>(s, half);
-#pragma unroll
-            for (int d = 0; d < DP / 32; ++d) dq[d] = mfma(col_frag<T, DP>(kt, 2 * t + half, d), ds, dq[d]);
-          }
+          for (int d = 0; d < DP / 16; ++d) s[n] = mfma(f[d], q[n][d], s[n]);
         }
+        fence();
+        row_frags<T, DP>(r, 1, t, f);
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+          dp[n] = 0.0f;
+#pragma unroll
+          for (int d = 0; d < DP / 16; ++d) dp[n] = mfma(f[d], go[n][d], dp[n]);
+        }
+        fence();
+        if (DP <= 64) col_frags<T, DP>(r, 0, t, kc);
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[n][r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], a.c, -lse[n]));
+          if (m != ~0ull) mask_scores(s[n], m, t, 0.0f);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[n][r] *= dp[n][r] - delta[n];
+          const V8 ds[2] = {to_frag<T>(s[n], 0), to_frag<T>(s[n], 1)};
+          if (DP > 64) {   // (the scores have been used up: their registers take the operands)
+            fence();
+            col_frags<T, DP>(r, 0, t, kc);
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d) dq[n][d] = mfma(kc[h][d], ds[h], dq[n][d]);
+        }
+        fence();
       });
-  if (!live) return;
-  if constexpr (SPLIT) {
-    float *p = a.part + ((split * (int64_t)a.B * a.E + be) * a.rows + row) * a.D;
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int at = 32 * d + 8 * r + 4 * hi;
-        const float x[4] = {dq[d][4 * r], dq[d][4 * r + 1], dq[d][4 * r + 2], dq[d][4 * r + 3]};
-        store_n<4>(p + at, a.D - at, x);
-      }
-  } else {
-    T *p = (T *)a.dq + (((int64_t)b * a.Lq + i) * a.H + h) * a.D;
-#pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int at = 32 * d + 8 * r + 4 * hi;
-        const float x[4] = {dq[d][4 * r] * a.scale, dq[d][4 * r + 1] * a.scale, dq[d][4 * r + 2] * a.scale, dq[d][4 * r + 3] * a.scale};
-        store_n<4>(p + at, a.D - at, x);
-      }
+  for (int n = 0; n < NS; ++n) {
+    const Column c = column_of(a, ct, n, 32 * NS);
+    if (!c.live) continue;
+    if constexpr (SPLIT) store_column<float, DP>(a.part + ((split * (int64_t)a.B * a.E + be) * a.rows + c.row) * a.D, a.D, dq[n], 1.0f);
+    else store_column<T, DP>((T *)a.dq + (((int64_t)b * a.Lq + c.i) * a.H + e * a.G + c.g) * a.D, a.D, dq[n], a.scale);
   }
 }
 
@@ -421,12 +631,175 @@ __global__ __launch_bounds__(kBlock) void k_attend_dq_join(AttArgs a) {
 }
 
 // ---- dK, dV ------------------------------------------------------------------------------------------------------
+//
+// Columns of 16 keys on v_mfma_f32_16x16x32, NK of them a wave: two sums of 16 x D leave the registers for two and more waves a SIMD where 32 keys
+// at D = 128 fill all of one.  A lane's scores are rows 16 b + 4 (lane / 16) + 0..3 of a sub-tile of 32 (b = 0, 1) of ONE key, which is the order
+// that the next product's operands take the rows in.
 
-template <typename T, int DP>
-__global__ __launch_bounds__(kBlock, DP <= 64 ? 2 : 1) void k_attend_dkv(AttArgs a) {
+template <typename T, int DP, int NK, int WAVES, bool WHOLE>
+__global__ __launch_bounds__(64 * WAVES, 2) void k_attend_dkv(AttArgs a) {
   typedef typename Vec<T>::type V8;
-  __shared__ __attribute__((aligned(16))) T qt[kTile * (DP + 8)], gt[kTile * (DP + 8)];
-  __shared__ __attribute__((aligned(16))) float lses[kTile], deltas[kTile];
+  typedef Reader<DP> R;
+  constexpr int kSize = Layout<DP>::kSize;
+  __shared__ __attribute__((aligned(256))) T tiles[2][2 * kSize];   // two buffers of a tile of q and a tile of dO
+  __shared__ __attribute__((aligned(16))) float stats[2][2][kTile];   // their lse and -delta
+  const int64_t item = work_item(a.work);
+  if (item >= a.work) return;
+  const int ct = (int)(item % a.col_tiles);
+  const int64_t be = item / a.col_tiles;
+  const int b = (int)(be / a.E), e = (int)(be - (int64_t)b * a.E);
+  const int wave = threadIdx.x >> 6;
+  const R reader = R::narrow(tiles);
+  V8 k[NK][DP / 32], v[NK][DP / 32];
+  f32x4 dk[NK][DP / 16], dv[NK][DP / 16];
+  bool on[NK], any = false, all = true;
+#pragma unroll
+  for (int j = 0; j < NK; ++j) {
+    const int lane = threadIdx.x & 63, key = ((ct * WAVES + wave) * NK + j) * 16 + (lane & 15);
+    on[j] = key < a.Lk && (!a.keep || a.keep[(int64_t)b * a.groups + group_of(a, key)] != 0);
+    const T *pk = (const T *)a.k + b * a.ks[0] + (int64_t)key * a.ks[1] + e * a.ks[2], *pv = (const T *)a.v + b * a.vs[0] + (int64_t)key * a.vs[1] + e * a.vs[2];
+#pragma unroll
+    for (int s = 0; s < DP / 32; ++s) {
+      const int at = 32 * s + 8 * (lane >> 4);
+      const u32x4 x = load16(pk + at, on[j] ? a.D - at : 0), y = load16(pv + at, on[j] ? a.D - at : 0);
+      __builtin_memcpy(&k[j][s], &x, 16), __builtin_memcpy(&v[j][s], &y, 16);
+    }
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) dk[j][d] = 0.0f, dv[j][d] = 0.0f;
+    any = any || on[j], all = all && on[j];
+  }
+  all = __all(all);
+  const T *qb = (const T *)a.q + b * a.qs[0] + (int64_t)e * a.G * a.qs[2], *gb = (const T *)a.go + b * a.gs[0] + (int64_t)e * a.G * a.gs[2];
+  Stage<T, DP, 64 * WAVES> staged;
+  float lse = 0.0f, delta = 0.0f;
+  const int n = !__syncthreads_or(any) ? 0 : WHOLE ? a.G * ((a.Lq + kTile - 1) / kTile) : (a.rows + kTile - 1) / kTile;   // (no kept key here: zeros)
+  // as in walk_tiles: a tile of q beside the first half of the work, a tile of dO beside the second
+  // the tile to load: with WHOLE from row i0 of head g0 (a head's last tile ends with it), else the rows from tile * kTile of the group's list
+  int g0 = 0, i0 = 0;
+  const auto load = [&](int which, int tile) {
+    const T *base = which ? gb : qb;
+    const int64_t stride = which ? a.gs[1] : a.qs[1], head = which ? a.gs[2] : a.qs[2];
+    const int at = WHOLE ? g0 * a.Lq + i0 : tile * kTile, left = (WHOLE ? a.Lq - i0 : a.rows - at);
+    if constexpr (WHOLE) {
+      staged.load(base + (int64_t)i0 * stride + g0 * head, (unsigned)stride, a.D, left < kTile ? left - 1 : kTile - 1);
+    } else {
+      staged.load_rows(a.D, [&](int r) -> const T * {
+        const int row = at + r, g = row / a.Lq;
+        return r < left ? base + (int64_t)(row - g * a.Lq) * stride + g * head : nullptr;
+      });
+    }
+    if (which == 0 && threadIdx.x < kTile) {
+      const bool there = (int)threadIdx.x < left;
+      const int64_t row = be * a.rows + at + (there ? threadIdx.x : 0);
+      const float x = a.lse[row], y = a.delta[row];
+      lse = there ? x : INFINITY, delta = y;   // (behind the last row: probabilities of 0)
+    }
+    if (WHOLE && which == 1 && (i0 += kTile) >= a.Lq) i0 = 0, ++g0;
+  };
+  const auto store = [&](int which, int buffer) {
+    staged.store(tiles[buffer] + which * kSize, ~0ull);
+    if (which == 0 && threadIdx.x < kTile) stats[buffer][0][threadIdx.x] = lse, stats[buffer][1][threadIdx.x] = -delta;
+  };
+  if (n) {
+    load(0, 0);
+    store(0, 0);
+    load(1, 0);
+    store(1, 0);
+  }
+  loads_done();
+  lds_barrier();
+  for (int tile = 0; tile < n; ++tile) {
+    const int buffer = tile & 1;
+    const R r = reader.at(buffer);
+    const int lane = threadIdx.x & 63;
+    if (tile + 1 < n) load(0, tile + 1);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      f32x4 s[NK][2], dp[NK][2];
+      V8 p[NK], ds[NK];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int j = 0; j < NK; ++j) s[j][h] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) {
+          const V8 f = R::template load<V8>((r.row ^ 64 * d) + (32 * t + 16 * h) * R::kRow);
+#pragma unroll
+          for (int j = 0; j < NK; ++j) s[j][h] = mfma16(f, k[j][d], s[j][h]);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const f32x4 from = *reinterpret_cast<const f32x4 *>(&stats[buffer][1][32 * t + 16 * h + 4 * (lane >> 4)]);   // dO v^T starts from -delta
+#pragma unroll
+        for (int j = 0; j < NK; ++j) dp[j][h] = from;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) {
+          const V8 f = R::template load<V8>((r.row ^ 64 * d) + R::kBytes + (32 * t + 16 * h) * R::kRow);
+#pragma unroll
+          for (int j = 0; j < NK; ++j) dp[j][h] = mfma16(f, v[j][d], dp[j][h]);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const f32x4 l = *reinterpret_cast<const f32x4 *>(&stats[buffer][0][32 * t + 16 * h + 4 * (lane >> 4)]);
+#pragma unroll
+        for (int j = 0; j < NK; ++j) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[j][h][r] = __builtin_amdgcn_exp2f(fmaf(s[j][h][r], a.c, -l[r]));
+          if (!all) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[j][h][r] = on[j] ? s[j][h][r] : 0.0f;
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            p[j][4 * h + r] = (T)s[j][h][r];
+            ds[j][4 * h + r] = (T)(s[j][h][r] * dp[j][h][r]);
+          }
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) {
+        const V8 f = R::template load_columns<V8>((r.col ^ 32 * d) + R::kBytes + 32 * t * R::kRow, (r.col ^ 32 * d) + R::kBytes + (32 * t + 16) * R::kRow);
+#pragma unroll
+        for (int j = 0; j < NK; ++j) dv[j][d] = mfma16(f, p[j], dv[j][d]);
+      }
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) {
+        const V8 f = R::template load_columns<V8>((r.col ^ 32 * d) + 32 * t * R::kRow, (r.col ^ 32 * d) + (32 * t + 16) * R::kRow);
+#pragma unroll
+        for (int j = 0; j < NK; ++j) dk[j][d] = mfma16(f, ds[j], dk[j][d]);
+      }
+      if (tile + 1 < n) {
+        store(t, buffer ^ 1);
+        if (t == 0) load(1, tile + 1);
+      }
+    }
+    lds_barrier();
+  }
+#pragma unroll
+  for (int j = 0; j < NK; ++j) {
+    const int lane = threadIdx.x & 63, key = ((ct * WAVES + wave) * NK + j) * 16 + (lane & 15);
+    if (key >= a.Lk) continue;
+    const int64_t to = (((int64_t)b * a.Lk + key) * a.E + e) * a.D;
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) {
+      const int at = 16 * d + 4 * (lane >> 4);
+      const float x[4] = {dk[j][d][0] * a.scale, dk[j][d][1] * a.scale, dk[j][d][2] * a.scale, dk[j][d][3] * a.scale};
+      const float y[4] = {dv[j][d][0], dv[j][d][1], dv[j][d][2], dv[j][d][3]};
+      store_n<4>((T *)a.dk + to + at, a.D - at, x);
+      store_n<4>((T *)a.dv + to + at, a.D - at, y);
+    }
+  }
+}
+
+
+template <typename T, int DP, bool WHOLE>
+__global__ __launch_bounds__(kBlock, 2) void k_attend_dkv32(AttArgs a) {
+  typedef typename Vec<T>::type V8;
+  constexpr int kSize = Layout<DP>::kSize;
+  __shared__ __attribute__((aligned(256))) T tiles[2][2 * kSize];   // two buffers of a tile of q and a tile of dO
+  __shared__ __attribute__((aligned(16))) float stats[2][2][kTile];   // their lse and -delta
   const int64_t item = work_item(a.work);
   if (item >= a.work) return;
   const int ct = (int)(item % a.col_tiles);
@@ -434,79 +807,119 @@ __global__ __launch_bounds__(kBlock, DP <= 64 ? 2 : 1) void k_attend_dkv(AttArgs
   const int b = (int)(be / a.E), e = (int)(be - (int64_t)b * a.E);
   const int lane = threadIdx.x & 63, hi = lane >> 5, wave = threadIdx.x >> 6;
   const int key = ct * (32 * kWaves) + wave * 32 + (lane & 31);
-  const bool there = key < a.Lk, on = there && (!a.keep || a.keep[(int64_t)b * a.groups + key / a.per] != 0);
+  const bool there = key < a.Lk, on = there && (!a.keep || a.keep[(int64_t)b * a.groups + group_of(a, key)] != 0);
   V8 k[DP / 16], v[DP / 16];
-  load_frags<T, DP>(on ? (const T *)a.k + b * a.ks[0] + (int64_t)key * a.ks[1] + e * a.ks[2] : nullptr, a.D, k);
-  load_frags<T, DP>(on ? (const T *)a.v + b * a.vs[0] + (int64_t)key * a.vs[1] + e * a.vs[2] : nullptr, a.D, v);
+  const auto key_frags = [&](const T *p, V8 (&f)[DP / 16]) {
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) {
+      const u32x4 r = load16(p + 16 * s + 8 * hi, on ? a.D - 16 * s - 8 * hi : 0);
+      __builtin_memcpy(&f[s], &r, 16);
+    }
+  };
+  key_frags((const T *)a.k + b * a.ks[0] + (int64_t)key * a.ks[1] + e * a.ks[2], k);
+  key_frags((const T *)a.v + b * a.vs[0] + (int64_t)key * a.vs[1] + e * a.vs[2], v);
   const bool all = __all(on);
   f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d) dk[d] = 0.0f, dv[d] = 0.0f;
   const T *qb = (const T *)a.q + b * a.qs[0] + (int64_t)e * a.G * a.qs[2], *gb = (const T *)a.go + b * a.gs[0] + (int64_t)e * a.G * a.gs[2];
-  Stage<T, DP> qs, gs;
+  Stage<T, DP> staged;
+  const Reader<DP> reader = Reader<DP>::wide(tiles);
   float lse = 0.0f, delta = 0.0f;
-  const int tiles = __syncthreads_or(on) ? (a.rows + kTile - 1) / kTile : 0;   // (no kept key here: zeros)
-  const auto load = [&](int tile) {
-    const int at = tile * kTile;
-    qs.load(a.D, [&](int r) -> const T * {
-      const int row = at + r, g = row / a.Lq;
-      return row < a.rows ? qb + (int64_t)(row - g * a.Lq) * a.qs[1] + g * a.qs[2] : nullptr;
-    });
-    gs.load(a.D, [&](int r) -> const T * {
-      const int row = at + r, g = row / a.Lq;
-      return row < a.rows ? gb + (int64_t)(row - g * a.Lq) * a.gs[1] + g * a.gs[2] : nullptr;
-    });
-    if (threadIdx.x < kTile) {
-      const int row = at + threadIdx.x;
-      lse = row < a.rows ? a.lse[be * a.rows + row] : INFINITY;
-      delta = row < a.rows ? a.delta[be * a.rows + row] : 0.0f;
+  const int n = !__syncthreads_or(on) ? 0 : WHOLE ? a.G * ((a.Lq + kTile - 1) / kTile) : (a.rows + kTile - 1) / kTile;   // (no kept key here: zeros)
+  // as in walk_tiles: a tile of q beside the first half of the work, a tile of dO beside the second
+  // the tile to load: with WHOLE from row i0 of head g0 (a head's last tile ends with it), else the rows from tile * kTile of the group's list
+  int g0 = 0, i0 = 0;
+  const auto load = [&](int which, int tile) {
+    const T *base = which ? gb : qb;
+    const int64_t stride = which ? a.gs[1] : a.qs[1], head = which ? a.gs[2] : a.qs[2];
+    const int at = WHOLE ? g0 * a.Lq + i0 : tile * kTile, left = (WHOLE ? a.Lq - i0 : a.rows - at);
+    if constexpr (WHOLE) {
+      staged.load(base + (int64_t)i0 * stride + g0 * head, (unsigned)stride, a.D, left < kTile ? left - 1 : kTile - 1);
+    } else {
+      staged.load_rows(a.D, [&](int r) -> const T * {
+        const int row = at + r, g = row / a.Lq;
+        return r < left ? base + (int64_t)(row - g * a.Lq) * stride + g * head : nullptr;
+      });
     }
+    if (which == 0 && threadIdx.x < kTile) {
+      const bool there = (int)threadIdx.x < left;
+      const int64_t row = be * a.rows + at + (there ? threadIdx.x : 0);
+      const float x = a.lse[row], y = a.delta[row];
+      lse = there ? x : INFINITY, delta = y;   // (behind the last row: probabilities of 0)
+    }
+    if (WHOLE && which == 1 && (i0 += kTile) >= a.Lq) i0 = 0, ++g0;
   };
-  if (tiles) load(0);
-  for (int tile = 0; tile < tiles; ++tile) {
-    lds_barrier();
-    qs.store(qt), gs.store(gt);
-    if (threadIdx.x < kTile) lses[threadIdx.x] = lse, deltas[threadIdx.x] = delta;
-    lds_barrier();
-    if (tile + 1 < tiles) load(tile + 1);
+  const auto store = [&](int which, int buffer) {
+    staged.store(tiles[buffer] + which * kSize, ~0ull);
+    if (which == 0 && threadIdx.x < kTile) stats[buffer][0][threadIdx.x] = lse, stats[buffer][1][threadIdx.x] = -delta;
+  };
+  if (n) {
+    load(0, 0);
+    store(0, 0);
+    load(1, 0);
+    store(1, 0);
+  }
+  loads_done();
+  lds_barrier();
+  for (int tile = 0; tile < n; ++tile) {
+    const int buffer = tile & 1;
+    const Reader<DP> r = reader.at(buffer);
+    if (tile + 1 < n) load(0, tile + 1);
+    V8 qf[DP / 16], gf[DP / 16], c[2][DP / 32];
+    row_frags<T, DP>(r, 0, 0, qf);
+    fence();
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      f32x16 s = 0.0f, dp = 0.0f;
+      f32x16 s = 0.0f, dp, l;
+      row_frags<T, DP>(r, 1, t, gf);
 #pragma unroll
-      for (int d = 0; d < DP / 16; ++d) s = mfma(row_frag<T, DP>(qt, t, d), k[d], s);
-#pragma unroll
-      for (int d = 0; d < DP / 16; ++d) dp = mfma(row_frag<T, DP>(gt, t, d), v[d], dp);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int at = 32 * t + 8 * (r / 4) + 4 * hi + r % 4;
-        float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lses[at]));
-        if (!all) p = on ? p : 0.0f;
-        s[r] = p;
-        dp[r] = p * (dp[r] - deltas[at]);
+      for (int r = 0; r < 4; ++r) {
+        const float4 x = *reinterpret_cast<const float4 *>(&stats[buffer][1][32 * t + 8 * r + 4 * hi]);
+        const float4 y = *reinterpret_cast<const float4 *>(&stats[buffer][0][32 * t + 8 * r + 4 * hi]);
+        dp[4 * r] = x.x, dp[4 * r + 1] = x.y, dp[4 * r + 2] = x.z, dp[4 * r + 3] = x.w;
+        l[4 * r] = y.x, l[4 * r + 1] = y.y, l[4 * r + 2] = y.z, l[4 * r + 3] = y.w;
       }
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const V8 p = to_frag<T>(s, half), ds = to_frag<T>(dp, half);
+      for (int d = 0; d < DP / 16; ++d) s = mfma(qf[d], k[d], s);
+      fence();
+      col_frags<T, DP>(r, 1, t, c);
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d) {
-          dv[d] = mfma(col_frag<T, DP>(gt, 2 * t + half, d), p, dv[d]);
-          dk[d] = mfma(col_frag<T, DP>(qt, 2 * t + half, d), ds, dk[d]);
-        }
+      for (int d = 0; d < DP / 16; ++d) dp = mfma(gf[d], v[d], dp);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -l[r]));
+      if (!all) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = on ? s[r] : 0.0f;
+      }
+      const V8 p[2] = {to_frag<T>(s, 0), to_frag<T>(s, 1)};
+      fence();
+      V8 c2[2][DP / 32];
+      col_frags<T, DP>(r, 0, t, c2);
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) dv[d] = mfma(c[half][d], p[half], dv[d]);
+      dp *= s;
+      const V8 ds[2] = {to_frag<T>(dp, 0), to_frag<T>(dp, 1)};
+      fence();
+      if (t == 0) row_frags<T, DP>(r, 0, 1, qf);
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) dk[d] = mfma(c2[half][d], ds[half], dk[d]);
+      fence();
+      if (tile + 1 < n) {
+        store(t, buffer ^ 1);
+        if (t == 0) load(1, tile + 1);
       }
     }
+    lds_barrier();
   }
   if (!there) return;
-  T *pk = (T *)a.dk + (((int64_t)b * a.Lk + key) * a.E + e) * a.D, *pv = (T *)a.dv + (((int64_t)b * a.Lk + key) * a.E + e) * a.D;
-#pragma unroll
-  for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int at = 32 * d + 8 * r + 4 * hi;
-      const float x[4] = {dk[d][4 * r] * a.scale, dk[d][4 * r + 1] * a.scale, dk[d][4 * r + 2] * a.scale, dk[d][4 * r + 3] * a.scale};
-      const float y[4] = {dv[d][4 * r], dv[d][4 * r + 1], dv[d][4 * r + 2], dv[d][4 * r + 3]};
-      store_n<4>(pk + at, a.D - at, x);
-      store_n<4>(pv + at, a.D - at, y);
-    }
+  const int64_t to = (((int64_t)b * a.Lk + key) * a.E + e) * a.D;
+  store_column<T, DP>((T *)a.dk + to, a.D, dk, a.scale);
+  store_column<T, DP>((T *)a.dv + to, a.D, dv, 1.0f);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------
@@ -526,11 +939,16 @@ int att_args(AttArgs &a, const mvr_attend_params *p) {
   a.B = p->batch, a.Lq = p->queries, a.Lk = p->keys, a.H = p->heads, a.E = p->kv_heads, a.G = p->heads / p->kv_heads, a.D = p->dim;
   a.groups = p->keep_groups, a.per = p->keep_groups ? p->keys / p->keep_groups : p->keys;
   a.rows = (int32_t)rows;
+  a.per_inverse = 1.0 / a.per;
   a.scale = p->scale, a.c = p->scale * 1.44269504088896340736f;
   for (int k = 0; k < 3; ++k) a.qs[k] = p->q_stride[k], a.ks[k] = p->k_stride[k], a.vs[k] = p->v_stride[k], a.gs[k] = p->grad_stride[k];
   a.tiles = (p->keys + kTile - 1) / kTile;
+  a.whole = p->dim % 8 == 0;
+  for (const int64_t *t : {a.qs, a.ks, a.vs, a.gs}) a.whole = a.whole && t[1] >= 0 && t[1] < 1 << 24;
+  // two columns of 32 queries a wave where heads leave the registers for it and there are queries enough
+  a.wide = a.whole && p->dim <= 64 && rows > 32 * kWaves;
   // few columns: the keys are dealt to several workgroups until there are about two per CU, each with four tiles at least
-  const int64_t cols = (rows + 32 * kWaves - 1) / (32 * kWaves), blocks = cols * a.B * a.E;
+  const int64_t per = 32 * kWaves * (1 + a.wide), cols = (rows + per - 1) / per, blocks = cols * a.B * a.E;
   int64_t splits = 512 / blocks, most = a.tiles / 4;
   splits = splits > most ? most : splits;
   a.splits = splits < 2 ? 1 : (int32_t)splits;
@@ -544,24 +962,32 @@ size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 size_t forward_bytes(const AttArgs &a) { return a.splits > 1 ? align256(lines(a) * a.splits * a.D * 4) + align256(lines(a) * a.splits * 4) : 0; }
 size_t backward_bytes(const AttArgs &a) { return align256(lines(a) * 4) + (a.splits > 1 ? align256(lines(a) * a.splits * a.D * 4) : 0); }
 
-// workgroups of 128 columns each, a multiple of 8 for work_item
-bool grid_of(AttArgs &a, int64_t columns, int splits, unsigned &blocks) {
-  a.col_tiles = (int32_t)((columns + 32 * kWaves - 1) / (32 * kWaves));
+// workgroups of `per` columns each, a multiple of 8 for work_item
+bool grid_of(AttArgs &a, int64_t columns, int per, int splits, unsigned &blocks) {
+  a.col_tiles = (int32_t)((columns + per - 1) / per);
   a.work = (int64_t)a.col_tiles * a.B * a.E * splits;
   const int64_t n = (a.work + 7) / 8 * 8;
   blocks = (unsigned)n;
   return n <= 0x7FFFFFFF;
 }
 
+// kernel<type, padded head, columns a wave, split, whole>
+#define MVR_ATT_COLUMNS(kernel, SPLIT, g, st, a)                                                                                  \
+  do {                                                                                                                            \
+    if ((a).wide) hipLaunchKernelGGL((kernel<T, DP, DP <= 64 ? 2 : 1, SPLIT, true>), g, dim3(kBlock), 0, st, a);                  \
+    else if ((a).whole) hipLaunchKernelGGL((kernel<T, DP, 1, SPLIT, true>), g, dim3(kBlock), 0, st, a);                           \
+    else hipLaunchKernelGGL((kernel<T, DP, 1, SPLIT, false>), g, dim3(kBlock), 0, st, a);                                         \
+  } while (0)
+
 template <typename T, int DP>
 int launch_forward(AttArgs a, hipStream_t st) {
   unsigned n;
-  if (!grid_of(a, a.rows, a.splits, n)) return bad("mvr_attend_tokens_forward: too many workgroups");
+  if (!grid_of(a, a.rows, 32 * kWaves * (1 + a.wide), a.splits, n)) return bad("mvr_attend_tokens_forward: too many workgroups");
   if (a.splits == 1) {
-    hipLaunchKernelGGL((k_attend<T, DP, false>), dim3(n), dim3(kBlock), 0, st, a);
+    MVR_ATT_COLUMNS(k_attend, false, dim3(n), st, a);
     return launched("k_attend");
   }
-  hipLaunchKernelGGL((k_attend<T, DP, true>), dim3(n), dim3(kBlock), 0, st, a);
+  MVR_ATT_COLUMNS(k_attend, true, dim3(n), st, a);
   if (int rc = launched("k_attend")) return rc;
   hipLaunchKernelGGL((k_attend_join<T>), dim3((unsigned)((lines(a) + kWaves - 1) / kWaves)), dim3(kBlock), 0, st, a);
   return launched("k_attend_join");
@@ -570,18 +996,28 @@ int launch_forward(AttArgs a, hipStream_t st) {
 template <typename T, int DP>
 int launch_backward(AttArgs a, hipStream_t st) {
   unsigned n;
-  if (!grid_of(a, a.rows, a.splits, n)) return bad("mvr_attend_tokens_backward: too many workgroups");
+  if (!grid_of(a, a.rows, 32 * kWaves * (1 + a.wide), a.splits, n)) return bad("mvr_attend_tokens_backward: too many workgroups");
   if (a.splits == 1) {
-    hipLaunchKernelGGL((k_attend_dq<T, DP, false>), dim3(n), dim3(kBlock), 0, st, a);
+    MVR_ATT_COLUMNS(k_attend_dq, false, dim3(n), st, a);
     if (int rc = launched("k_attend_dq")) return rc;
   } else {
-    hipLaunchKernelGGL((k_attend_dq<T, DP, true>), dim3(n), dim3(kBlock), 0, st, a);
+    MVR_ATT_COLUMNS(k_attend_dq, true, dim3(n), st, a);
     if (int rc = launched("k_attend_dq")) return rc;
     hipLaunchKernelGGL((k_attend_dq_join<T>), dim3((unsigned)((lines(a) + kWaves - 1) / kWaves)), dim3(kBlock), 0, st, a);
     if (int rc = launched("k_attend_dq_join")) return rc;
   }
-  if (!grid_of(a, a.Lk, 1, n)) return bad("mvr_attend_tokens_backward: too many workgroups");
-  hipLaunchKernelGGL((k_attend_dkv<T, DP>), dim3(n), dim3(kBlock), 0, st, a);
+  // a group's heads of fewer queries than a tile holds share tiles
+  const bool whole = a.whole && (a.G == 1 || a.Lq >= kTile);
+  constexpr int kKeys = DP <= 64 ? 32 * kWaves : 16 * kWaves;
+  if (!grid_of(a, a.Lk, kKeys, 1, n)) return bad("mvr_attend_tokens_backward: too many workgroups");
+  const dim3 g(n), blk(kBlock);
+  if constexpr (DP <= 64) {
+    if (whole) hipLaunchKernelGGL((k_attend_dkv32<T, DP, true>), g, blk, 0, st, a);
+    else hipLaunchKernelGGL((k_attend_dkv32<T, DP, false>), g, blk, 0, st, a);
+  } else {
+    if (whole) hipLaunchKernelGGL((k_attend_dkv<T, DP, 1, kWaves, true>), g, blk, 0, st, a);
+    else hipLaunchKernelGGL((k_attend_dkv<T, DP, 1, kWaves, false>), g, blk, 0, st, a);
+  }
   return launched("k_attend_dkv");
 }
 
