@@ -418,69 +418,67 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend(AttArgs a) {
   const Reader<DP> reader = Reader<DP>::wide(tiles);
   const int first = SPLIT ? split * a.split_tiles : 0, last = SPLIT && first + a.split_tiles < a.tiles ? first + a.split_tiles : a.tiles;
   f32x16 s[NS][2];
-  walk_tiles(
-      a, b, first, last,
-      MVR_ATT_KV,
-      [&](int buffer, unsigned long long m, int half) {
-        const Reader<DP> r = reader.at(buffer);
-        if (half == 1) {   // probabilities and their product with v
+  const auto step = [&](int buffer, unsigned long long m, int half) {
+    const Reader<DP> r = reader.at(buffer);
+    if (half == 1) {   // probabilities and their product with v
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            V8 v[2][DP / 32], p[NS][2];
-            col_frags<T, DP>(r, 1, t, v);
-#pragma unroll
-            for (int n = 0; n < NS; ++n) {
-              const float off = top[n] == -INFINITY ? 0.0f : top[n];
-#pragma unroll
-              for (int r = 0; r < 16; ++r) s[n][t][r] = __builtin_amdgcn_exp2f(fmaf(s[n][t][r], a.c, -off));
-              p[n][0] = to_frag<T>(s[n][t], 0), p[n][1] = to_frag<T>(s[n][t], 1);
-              sum[n] = add_frag(p[n][1], add_frag(p[n][0], sum[n]));   // (of the probabilities as they enter the product)
-#pragma unroll
-              for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int d = 0; d < DP / 32; ++d) o[n][d] = mfma(v[h][d], p[n][h], o[n][d]);
-            }
-          }
-          return;
-        }
-        // scores, running maximum
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          V8 k[DP / 16];
-          row_frags<T, DP>(r, 0, t, k);
-#pragma unroll
-          for (int n = 0; n < NS; ++n) {
-            s[n][t] = 0.0f;
-#pragma unroll
-            for (int d = 0; d < DP / 16; ++d) s[n][t] = mfma(k[d], q[n][d], s[n][t]);
-          }
-        }
-        if (m != ~0ull) {
-#pragma unroll
-          for (int n = 0; n < NS; ++n) mask_scores(s[n][0], m, 0, -INFINITY), mask_scores(s[n][1], m, 1, -INFINITY);
-        }
-        float now[NS];
-        bool up = false;
+      for (int t = 0; t < 2; ++t) {
+        V8 v[2][DP / 32], p[NS][2];
+        col_frags<T, DP>(r, 1, t, v);
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
-          float mx = fmaxf(s[n][0][0], s[n][1][0]);
+          const float off = top[n] == -INFINITY ? 0.0f : top[n];
 #pragma unroll
-          for (int r = 1; r < 16; ++r) mx = fmaxf(fmaxf(s[n][0][r], s[n][1][r]), mx);
-          mx = fmaxf(mx, other_half(mx));
-          now[n] = fmaxf(top[n], mx * a.c);
-          up = up || now[n] > top[n] + kSlack;
+          for (int r = 0; r < 16; ++r) s[n][t][r] = __builtin_amdgcn_exp2f(fmaf(s[n][t][r], a.c, -off));
+          p[n][0] = to_frag<T>(s[n][t], 0), p[n][1] = to_frag<T>(s[n][t], 1);
+          sum[n] = add_frag(p[n][1], add_frag(p[n][0], sum[n]));   // (of the probabilities as they enter the product)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d) o[n][d] = mfma(v[h][d], p[n][h], o[n][d]);
         }
-        if (__any(up)) {
+      }
+      return;
+    }
+    // scores, running maximum
 #pragma unroll
-          for (int n = 0; n < NS; ++n) {
-            const float f = __builtin_amdgcn_exp2f(top[n] - (now[n] == -INFINITY ? 0.0f : now[n]));
-            sum[n] *= f;
+    for (int t = 0; t < 2; ++t) {
+      V8 k[DP / 16];
+      row_frags<T, DP>(r, 0, t, k);
 #pragma unroll
-            for (int d = 0; d < DP / 32; ++d) o[n][d] *= f;
-            top[n] = now[n];
-          }
-        }
-      });
+      for (int n = 0; n < NS; ++n) {
+        s[n][t] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d) s[n][t] = mfma(k[d], q[n][d], s[n][t]);
+      }
+    }
+    if (m != ~0ull) {
+#pragma unroll
+      for (int n = 0; n < NS; ++n) mask_scores(s[n][0], m, 0, -INFINITY), mask_scores(s[n][1], m, 1, -INFINITY);
+    }
+    float now[NS];
+    bool up = false;
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+      float mx = fmaxf(s[n][0][0], s[n][1][0]);
+#pragma unroll
+      for (int r = 1; r < 16; ++r) mx = fmaxf(fmaxf(s[n][0][r], s[n][1][r]), mx);
+      mx = fmaxf(mx, other_half(mx));
+      now[n] = fmaxf(top[n], mx * a.c);
+      up = up || now[n] > top[n] + kSlack;
+    }
+    if (__any(up)) {
+#pragma unroll
+      for (int n = 0; n < NS; ++n) {
+        const float f = __builtin_amdgcn_exp2f(top[n] - (now[n] == -INFINITY ? 0.0f : now[n]));
+        sum[n] *= f;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) o[n][d] *= f;
+        top[n] = now[n];
+      }
+    }
+  };
+  walk_tiles(a, b, first, last, MVR_ATT_KV, step);
   const int hi = (threadIdx.x & 63) >> 5;
 #pragma unroll
   for (int n = 0; n < NS; ++n) {
@@ -525,7 +523,10 @@ __global__ __launch_bounds__(kBlock) void k_attend_join(AttArgs a) {
 
 // ---- dQ (and delta) ----------------------------------------------------------------------------------------------
 
-template <typename T, int DP, int NS, bool SPLIT, bool WHOLE>
+// One column of 32 queries a wave: with heads of 64 160 registers and three waves a SIMD, where two columns take 246 and leave two.
+// 16 x 2352 tokens, 12 heads of 64, 12 views of which a quarter is dropped, bfloat16: 424 us against 472 with two; the forward, which keeps less
+// per column, takes 364 us with two and 411 with one.
+template <typename T, int DP, bool SPLIT, bool WHOLE>
 __global__ __launch_bounds__(kBlock, 2) void k_attend_dq(AttArgs a) {
   typedef typename Vec<T>::type V8;
   constexpr int kSize = Layout<DP>::kSize;
@@ -537,81 +538,61 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dq(AttArgs a) {
   const int ct = (int)(item % a.col_tiles);
   const int64_t be = item / a.col_tiles;
   const int b = (int)(be / a.E), e = (int)(be - (int64_t)b * a.E);
-  V8 q[NS][DP / 16], go[NS][DP / 16];
-  f32x16 dq[NS][DP / 32];
-  float lse[NS], delta[NS];
+  V8 q[DP / 16], go[DP / 16];
+  f32x16 dq[DP / 32];
+  const Column c = column_of(a, ct, 0, 32);
+  const int h = e * a.G + c.g;
+  float lse, delta = 0.0f;
+  load_frags<T, DP>((const T *)a.q + b * a.qs[0] + c.i * a.qs[1] + h * a.qs[2], a, q);
+  load_frags<T, DP>((const T *)a.go + b * a.gs[0] + c.i * a.gs[1] + h * a.gs[2], a, go);
+  V8 o[DP / 16];
+  load_frags<T, DP>((const T *)a.o + (((int64_t)b * a.Lq + c.i) * a.H + h) * a.D, a, o);
 #pragma unroll
-  for (int n = 0; n < NS; ++n) {
-    const Column c = column_of(a, ct, n, 32 * NS);
-    const int h = e * a.G + c.g;
-    load_frags<T, DP>((const T *)a.q + b * a.qs[0] + c.i * a.qs[1] + h * a.qs[2], a, q[n]);
-    load_frags<T, DP>((const T *)a.go + b * a.gs[0] + c.i * a.gs[1] + h * a.gs[2], a, go[n]);
-    V8 o[DP / 16];
-    load_frags<T, DP>((const T *)a.o + (((int64_t)b * a.Lq + c.i) * a.H + h) * a.D, a, o);
-    delta[n] = 0.0f;
+  for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
-    for (int s = 0; s < DP / 16; ++s)
+    for (int k = 0; k < 8; ++k) delta += (float)o[s][k] * (float)go[s][k];
+  delta += other_half(delta);
+  lse = c.live ? a.lse[be * a.rows + c.row] : INFINITY;
+  if (c.live && (threadIdx.x & 32) == 0 && split == 0) a.delta[be * a.rows + c.row] = delta;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) delta[n] += (float)o[s][k] * (float)go[n][s][k];
-    delta[n] += other_half(delta[n]);
-    lse[n] = c.live ? a.lse[be * a.rows + c.row] : INFINITY;
-    if (c.live && (threadIdx.x & 32) == 0 && split == 0) a.delta[be * a.rows + c.row] = delta[n];
-#pragma unroll
-    for (int d = 0; d < DP / 32; ++d) dq[n][d] = 0.0f;
-  }
+  for (int d = 0; d < DP / 32; ++d) dq[d] = 0.0f;
   const T *kb = (const T *)a.k + b * a.ks[0] + e * a.ks[2], *vb = (const T *)a.v + b * a.vs[0] + e * a.vs[2];
   Stage<T, DP> staged;
   const Reader<DP> reader = Reader<DP>::wide(tiles);
   const int first = SPLIT ? split * a.split_tiles : 0, last = SPLIT && first + a.split_tiles < a.tiles ? first + a.split_tiles : a.tiles;
-  walk_tiles(
-      a, b, first, last,
-      MVR_ATT_KV,
-      [&](int buffer, unsigned long long m, int t) {
-        const Reader<DP> r = reader.at(buffer);
-        V8 f[DP / 16], kc[2][DP / 32];
-        f32x16 s[NS], dp[NS];
-        row_frags<T, DP>(r, 0, t, f);
+  const auto step = [&](int buffer, unsigned long long m, int t) {
+    const Reader<DP> r = reader.at(buffer);
+    V8 f[DP / 16], kc[2][DP / 32];
+    f32x16 s = 0.0f, dp = 0.0f;
+    row_frags<T, DP>(r, 0, t, f);
 #pragma unroll
-        for (int n = 0; n < NS; ++n) {
-          s[n] = 0.0f;
+    for (int d = 0; d < DP / 16; ++d) s = mfma(f[d], q[d], s);
+    fence();
+    row_frags<T, DP>(r, 1, t, f);
 #pragma unroll
-          for (int d = 0; d < DP / 16; ++d) s[n] = mfma(f[d], q[n][d], s[n]);
-        }
-        fence();
-        row_frags<T, DP>(r, 1, t, f);
+    for (int d = 0; d < DP / 16; ++d) dp = mfma(f[d], go[d], dp);
+    fence();
+    if (DP <= 64) col_frags<T, DP>(r, 0, t, kc);
 #pragma unroll
-        for (int n = 0; n < NS; ++n) {
-          dp[n] = 0.0f;
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse));
+    if (m != ~0ull) mask_scores(s, m, t, 0.0f);
 #pragma unroll
-          for (int d = 0; d < DP / 16; ++d) dp[n] = mfma(f[d], go[n][d], dp[n]);
-        }
-        fence();
-        if (DP <= 64) col_frags<T, DP>(r, 0, t, kc);
+    for (int r = 0; r < 16; ++r) s[r] *= dp[r] - delta;
+    const V8 ds[2] = {to_frag<T>(s, 0), to_frag<T>(s, 1)};
+    if (DP > 64) {   // (the scores have been used up: their registers take the operands)
+      fence();
+      col_frags<T, DP>(r, 0, t, kc);
+    }
 #pragma unroll
-        for (int n = 0; n < NS; ++n) {
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[n][r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], a.c, -lse[n]));
-          if (m != ~0ull) mask_scores(s[n], m, t, 0.0f);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[n][r] *= dp[n][r] - delta[n];
-          const V8 ds[2] = {to_frag<T>(s[n], 0), to_frag<T>(s[n], 1)};
-          if (DP > 64) {   // (the scores have been used up: their registers take the operands)
-            fence();
-            col_frags<T, DP>(r, 0, t, kc);
-          }
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int d = 0; d < DP / 32; ++d) dq[n][d] = mfma(kc[h][d], ds[h], dq[n][d]);
-        }
-        fence();
-      });
-#pragma unroll
-  for (int n = 0; n < NS; ++n) {
-    const Column c = column_of(a, ct, n, 32 * NS);
-    if (!c.live) continue;
-    if constexpr (SPLIT) store_column<float, DP>(a.part + ((split * (int64_t)a.B * a.E + be) * a.rows + c.row) * a.D, a.D, dq[n], 1.0f);
-    else store_column<T, DP>((T *)a.dq + (((int64_t)b * a.Lq + c.i) * a.H + e * a.G + c.g) * a.D, a.D, dq[n], a.scale);
+      for (int d = 0; d < DP / 32; ++d) dq[d] = mfma(kc[h][d], ds[h], dq[d]);
+    fence();
+  };
+  walk_tiles(a, b, first, last, MVR_ATT_KV, step);
+  if (c.live) {
+    if constexpr (SPLIT) store_column<float, DP>(a.part + ((split * (int64_t)a.B * a.E + be) * a.rows + c.row) * a.D, a.D, dq, 1.0f);
+    else store_column<T, DP>((T *)a.dq + (((int64_t)b * a.Lq + c.i) * a.H + e * a.G + c.g) * a.D, a.D, dq, a.scale);
   }
 }
 
@@ -971,23 +952,21 @@ bool grid_of(AttArgs &a, int64_t columns, int per, int splits, unsigned &blocks)
   return n <= 0x7FFFFFFF;
 }
 
-// kernel<type, padded head, columns a wave, split, whole>
-#define MVR_ATT_COLUMNS(kernel, SPLIT, g, st, a)                                                                                  \
-  do {                                                                                                                            \
-    if ((a).wide) hipLaunchKernelGGL((kernel<T, DP, DP <= 64 ? 2 : 1, SPLIT, true>), g, dim3(kBlock), 0, st, a);                  \
-    else if ((a).whole) hipLaunchKernelGGL((kernel<T, DP, 1, SPLIT, true>), g, dim3(kBlock), 0, st, a);                           \
-    else hipLaunchKernelGGL((kernel<T, DP, 1, SPLIT, false>), g, dim3(kBlock), 0, st, a);                                         \
-  } while (0)
-
 template <typename T, int DP>
 int launch_forward(AttArgs a, hipStream_t st) {
   unsigned n;
   if (!grid_of(a, a.rows, 32 * kWaves * (1 + a.wide), a.splits, n)) return bad("mvr_attend_tokens_forward: too many workgroups");
+  const dim3 g(n), blk(kBlock);
+  constexpr int kWide = DP <= 64 ? 2 : 1;
   if (a.splits == 1) {
-    MVR_ATT_COLUMNS(k_attend, false, dim3(n), st, a);
+    if (a.wide) hipLaunchKernelGGL((k_attend<T, DP, kWide, false, true>), g, blk, 0, st, a);
+    else if (a.whole) hipLaunchKernelGGL((k_attend<T, DP, 1, false, true>), g, blk, 0, st, a);
+    else hipLaunchKernelGGL((k_attend<T, DP, 1, false, false>), g, blk, 0, st, a);
     return launched("k_attend");
   }
-  MVR_ATT_COLUMNS(k_attend, true, dim3(n), st, a);
+  if (a.wide) hipLaunchKernelGGL((k_attend<T, DP, kWide, true, true>), g, blk, 0, st, a);
+  else if (a.whole) hipLaunchKernelGGL((k_attend<T, DP, 1, true, true>), g, blk, 0, st, a);
+  else hipLaunchKernelGGL((k_attend<T, DP, 1, true, false>), g, blk, 0, st, a);
   if (int rc = launched("k_attend")) return rc;
   hipLaunchKernelGGL((k_attend_join<T>), dim3((unsigned)((lines(a) + kWaves - 1) / kWaves)), dim3(kBlock), 0, st, a);
   return launched("k_attend_join");
@@ -996,13 +975,16 @@ int launch_forward(AttArgs a, hipStream_t st) {
 template <typename T, int DP>
 int launch_backward(AttArgs a, hipStream_t st) {
   unsigned n;
-  if (!grid_of(a, a.rows, 32 * kWaves * (1 + a.wide), a.splits, n)) return bad("mvr_attend_tokens_backward: too many workgroups");
+  if (!grid_of(a, a.rows, 32 * kWaves, a.splits, n)) return bad("mvr_attend_tokens_backward: too many workgroups");
   if (a.splits == 1) {
-    MVR_ATT_COLUMNS(k_attend_dq, false, dim3(n), st, a);
-    if (int rc = launched("k_attend_dq")) return rc;
+    if (a.whole) hipLaunchKernelGGL((k_attend_dq<T, DP, false, true>), dim3(n), dim3(kBlock), 0, st, a);
+    else hipLaunchKernelGGL((k_attend_dq<T, DP, false, false>), dim3(n), dim3(kBlock), 0, st, a);
   } else {
-    MVR_ATT_COLUMNS(k_attend_dq, true, dim3(n), st, a);
-    if (int rc = launched("k_attend_dq")) return rc;
+    if (a.whole) hipLaunchKernelGGL((k_attend_dq<T, DP, true, true>), dim3(n), dim3(kBlock), 0, st, a);
+    else hipLaunchKernelGGL((k_attend_dq<T, DP, true, false>), dim3(n), dim3(kBlock), 0, st, a);
+  }
+  if (int rc = launched("k_attend_dq")) return rc;
+  if (a.splits > 1) {
     hipLaunchKernelGGL((k_attend_dq_join<T>), dim3((unsigned)((lines(a) + kWaves - 1) / kWaves)), dim3(kBlock), 0, st, a);
     if (int rc = launched("k_attend_dq_join")) return rc;
   }
