@@ -475,8 +475,8 @@ int mvr_add_norm_tokens_backward(const mvr_norm_params *params, const void *y, c
 
 /* Attention over tokens: out = softmax(scale q k^T over the kept keys) v, head by head; 16-bit tensors, heads of at most 128.
  * heads is a multiple of kv_heads (consecutive heads share a key/value head).  keep: (batch, keep_groups) bytes, each for
- * keys / keep_groups consecutive keys (one per view; non-zero: kept); a key that is not kept is not read.  A query without any
- * kept key gets 0 and passes no gradient on. */
+ * keys / keep_groups consecutive keys (one per view; non-zero: kept); of a key that is not kept nothing enters any result, whatever it
+ * holds.  A query without any kept key gets 0 and passes no gradient on. */
 typedef struct mvr_attend_params {
   int32_t batch, queries, keys, heads, kv_heads, dim;
   int32_t type;            /* MVR_TYPE_HALF or MVR_TYPE_BFLOAT: of every tensor but lse */

@@ -3,9 +3,9 @@
 //   dV = P^T dO,  dS = P (dO v^T - delta),  delta = rowsum(dO O),  dQ = scale dS k,  dK = scale dS^T q
 // One pass over the keys with the running maximum and sum; nothing of size queries x keys is ever stored: the backward recomputes the
 // probabilities from q, k and lse.  Sums, maxima and exponentials are 32 bits wide; P and dS are rounded to the tensors' type where they
-// enter a matrix instruction (P lies in [0, 1] and dS enters as a factor: half a step of the type relative to each, as of the inputs).
+// enter a matrix instruction: half a step of the type relative to each, as of the inputs.  (The forward's P lies in [0, 2^8], as its maximum may lag.)
 //
-// All three kernels have one shape.  A wave owns 32 columns — queries (forward, dQ) or keys (dK/dV) — and walks the other side in tiles that its
+// All three kernels have one shape.  A wave owns columns — queries (forward: two times 32 or 32, dQ: 32) or keys (dK/dV: 32 or 16) — and walks the other side in tiles that its
 // workgroup stages in LDS.  Scores come as tile x columns from v_mfma_f32_32x32x16: a lane then holds 16 scores of ONE column (rows 8 (r / 4) +
 // 4 (lane / 32) + r % 4), so softmax statistics need one exchange between the wave's halves, and eight consecutive registers are, with the
 // tile's rows taken in that same order, an operand of the next product: probabilities never leave the registers.  The other operand of
@@ -94,11 +94,10 @@ struct Layout {
 };
 
 // A tile of kTile rows on its way from memory to LDS
-template <typename T, int DP, int THREADS = kBlock>
+template <typename T, int DP>
 struct Stage {
-  static constexpr int kPerRow = DP / 8, kChunks = (kTile * kPerRow + THREADS - 1) / THREADS;
-  static constexpr bool kEven = THREADS % kPerRow == 0;   // a thread's chunks lie in one column, THREADS / kPerRow rows apart
-  static constexpr bool kPart = kTile * kPerRow % THREADS != 0;   // the last chunk is not for every thread
+  static constexpr int kPerRow = DP / 8, kChunks = kTile * kPerRow / kBlock;   // (a whole number for 32, 64, 96 and 128)
+  static constexpr bool kEven = kBlock % kPerRow == 0;   // a thread's chunks lie in one column, kBlock / kPerRow rows apart
   u32x4 r[kChunks];
   __device__ __forceinline__ Stage() {
 #pragma unroll
@@ -107,7 +106,7 @@ struct Stage {
   // D a multiple of 8, rows `stride` elements apart, the last of them again for what lies behind it: one way for whole tiles and ends, as loads
   // on two ways into the same registers are copied, and waited for, where the ways meet
   __device__ __forceinline__ void load(const T *base, unsigned stride, int D, unsigned last) {
-    if constexpr (kEven && !kPart) {
+    if constexpr (kEven) {
       const unsigned i = threadIdx.x / kPerRow, c = threadIdx.x % kPerRow * 8;
       if (c < (unsigned)D) {   // (chunks behind a head stay the zeros they are)
         unsigned at = i * stride + c;
@@ -115,15 +114,15 @@ struct Stage {
         asm volatile("" : "+v"(at));   // (one address is kept through the loop, not one per chunk)
 #pragma unroll
         for (int k = 0; k < kChunks; ++k) {
-          const unsigned x = at + k * (THREADS / kPerRow) * stride;
+          const unsigned x = at + k * (kBlock / kPerRow) * stride;
           __builtin_memcpy(&r[k], base + (x < end ? x : end), 16);
         }
       }
     } else {
 #pragma unroll
       for (int k = 0; k < kChunks; ++k) {
-        const unsigned e = threadIdx.x + k * THREADS, i = e / kPerRow, c = e % kPerRow * 8;
-        if (c < (unsigned)D && (!kPart || i < kTile)) __builtin_memcpy(&r[k], base + (i < last ? i : last) * stride + c, 16);
+        const unsigned e = threadIdx.x + k * kBlock, i = e / kPerRow, c = e % kPerRow * 8;
+        if (c < (unsigned)D) __builtin_memcpy(&r[k], base + (i < last ? i : last) * stride + c, 16);
       }
     }
   }
@@ -134,8 +133,8 @@ struct Stage {
     asm volatile("" : "+v"(tid));   // (its addresses are not to be kept in registers all through the loop)
 #pragma unroll
     for (int k = 0; k < kChunks; ++k) {
-      const int e = tid + k * THREADS, i = e / kPerRow, c = e % kPerRow * 8;
-      const T *p = kPart && i >= kTile ? nullptr : row(i);
+      const int e = tid + k * kBlock, i = e / kPerRow, c = e % kPerRow * 8;
+      const T *p = row(i);
       r[k] = load16(p + c, p ? D - c : 0);
     }
   }
@@ -144,13 +143,13 @@ struct Stage {
     const int i0 = threadIdx.x / kPerRow, at0 = i0 * Layout<DP>::kPitch + (threadIdx.x % kPerRow ^ Layout<DP>::swizzle(i0)) * 8;
 #pragma unroll
     for (int k = 0; k < kChunks; ++k) {
-      const int e = threadIdx.x + k * THREADS, i = e / kPerRow;
+      const int e = threadIdx.x + k * kBlock, i = e / kPerRow;
       u32x4 x = r[k];
       if (rows != ~0ull && !(rows >> (i & 63) & 1)) x = u32x4{0, 0, 0, 0};
       // (whole multiples of 16 rows apart the swizzle is the same)
-      const int at = kEven && THREADS / kPerRow % 16 == 0 ? at0 + k * (THREADS / kPerRow) * Layout<DP>::kPitch
+      const int at = kEven && kBlock / kPerRow % 16 == 0 ? at0 + k * (kBlock / kPerRow) * Layout<DP>::kPitch
                                                           : i * Layout<DP>::kPitch + (e % kPerRow ^ Layout<DP>::swizzle(i)) * 8;
-      if (!kPart || i < kTile) *reinterpret_cast<u32x4 *>(lds + at) = x;
+      *reinterpret_cast<u32x4 *>(lds + at) = x;
     }
   }
 };
@@ -613,12 +612,12 @@ __global__ __launch_bounds__(kBlock) void k_attend_dq_join(AttArgs a) {
 
 // ---- dK, dV ------------------------------------------------------------------------------------------------------
 //
-// Columns of 16 keys on v_mfma_f32_16x16x32, NK of them a wave: two sums of 16 x D leave the registers for two and more waves a SIMD where 32 keys
-// at D = 128 fill all of one.  A lane's scores are rows 16 b + 4 (lane / 16) + 0..3 of a sub-tile of 32 (b = 0, 1) of ONE key, which is the order
+// Heads above 64: a column of 16 keys a wave on v_mfma_f32_16x16x32, whose two sums of 16 x D leave the registers for two waves a SIMD, where 32
+// keys of 128 fill all of one.  A lane's scores are rows 16 b + 4 (lane / 16) + 0..3 of a sub-tile of 32 (b = 0, 1) of ONE key, which is the order
 // that the next product's operands take the rows in.
 
-template <typename T, int DP, int NK, int WAVES, bool WHOLE>
-__global__ __launch_bounds__(64 * WAVES, 2) void k_attend_dkv(AttArgs a) {
+template <typename T, int DP, bool WHOLE>
+__global__ __launch_bounds__(kBlock, 2) void k_attend_dkv16(AttArgs a) {
   typedef typename Vec<T>::type V8;
   typedef Reader<DP> R;
   constexpr int kSize = Layout<DP>::kSize;
@@ -631,29 +630,24 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attend_dkv(AttArgs a) {
   const int b = (int)(be / a.E), e = (int)(be - (int64_t)b * a.E);
   const int wave = threadIdx.x >> 6;
   const R reader = R::narrow(tiles);
-  V8 k[NK][DP / 32], v[NK][DP / 32];
-  f32x4 dk[NK][DP / 16], dv[NK][DP / 16];
-  bool on[NK], any = false, all = true;
+  V8 k[DP / 32], v[DP / 32];
+  f32x4 dk[DP / 16], dv[DP / 16];
+  const int lane = threadIdx.x & 63, key = (ct * kWaves + wave) * 16 + (lane & 15);
+  const bool there = key < a.Lk, on = there && (!a.keep || a.keep[(int64_t)b * a.groups + group_of(a, key)] != 0);
+  const T *pk = (const T *)a.k + b * a.ks[0] + (int64_t)key * a.ks[1] + e * a.ks[2], *pv = (const T *)a.v + b * a.vs[0] + (int64_t)key * a.vs[1] + e * a.vs[2];
 #pragma unroll
-  for (int j = 0; j < NK; ++j) {
-    const int lane = threadIdx.x & 63, key = ((ct * WAVES + wave) * NK + j) * 16 + (lane & 15);
-    on[j] = key < a.Lk && (!a.keep || a.keep[(int64_t)b * a.groups + group_of(a, key)] != 0);
-    const T *pk = (const T *)a.k + b * a.ks[0] + (int64_t)key * a.ks[1] + e * a.ks[2], *pv = (const T *)a.v + b * a.vs[0] + (int64_t)key * a.vs[1] + e * a.vs[2];
-#pragma unroll
-    for (int s = 0; s < DP / 32; ++s) {
-      const int at = 32 * s + 8 * (lane >> 4);
-      const u32x4 x = load16(pk + at, on[j] ? a.D - at : 0), y = load16(pv + at, on[j] ? a.D - at : 0);
-      __builtin_memcpy(&k[j][s], &x, 16), __builtin_memcpy(&v[j][s], &y, 16);
-    }
-#pragma unroll
-    for (int d = 0; d < DP / 16; ++d) dk[j][d] = 0.0f, dv[j][d] = 0.0f;
-    any = any || on[j], all = all && on[j];
+  for (int s = 0; s < DP / 32; ++s) {
+    const int at = 32 * s + 8 * (lane >> 4);
+    const u32x4 x = load16(pk + at, on ? a.D - at : 0), y = load16(pv + at, on ? a.D - at : 0);
+    __builtin_memcpy(&k[s], &x, 16), __builtin_memcpy(&v[s], &y, 16);
   }
-  all = __all(all);
+#pragma unroll
+  for (int d = 0; d < DP / 16; ++d) dk[d] = 0.0f, dv[d] = 0.0f;
+  const bool all = __all(on);
   const T *qb = (const T *)a.q + b * a.qs[0] + (int64_t)e * a.G * a.qs[2], *gb = (const T *)a.go + b * a.gs[0] + (int64_t)e * a.G * a.gs[2];
-  Stage<T, DP, 64 * WAVES> staged;
+  Stage<T, DP> staged;
   float lse = 0.0f, delta = 0.0f;
-  const int n = !__syncthreads_or(any) ? 0 : WHOLE ? a.G * ((a.Lq + kTile - 1) / kTile) : (a.rows + kTile - 1) / kTile;   // (no kept key here: zeros)
+  const int n = !__syncthreads_or(on) ? 0 : WHOLE ? a.G * ((a.Lq + kTile - 1) / kTile) : (a.rows + kTile - 1) / kTile;   // (no kept key here: zeros)
   // as in walk_tiles: a tile of q beside the first half of the work, a tile of dO beside the second
   // the tile to load: with WHOLE from row i0 of head g0 (a head's last tile ends with it), else the rows from tile * kTile of the group's list
   int g0 = 0, i0 = 0;
@@ -670,10 +664,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attend_dkv(AttArgs a) {
       });
     }
     if (which == 0 && threadIdx.x < kTile) {
-      const bool there = (int)threadIdx.x < left;
-      const int64_t row = be * a.rows + at + (there ? threadIdx.x : 0);
+      const bool in = (int)threadIdx.x < left;
+      const int64_t row = be * a.rows + at + (in ? threadIdx.x : 0);
       const float x = a.lse[row], y = a.delta[row];
-      lse = there ? x : INFINITY, delta = y;   // (behind the last row: probabilities of 0)
+      lse = in ? x : INFINITY, delta = y;   // (behind the last row: probabilities of 0)
     }
     if (WHOLE && which == 1 && (i0 += kTile) >= a.Lq) i0 = 0, ++g0;
   };
@@ -692,64 +686,54 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attend_dkv(AttArgs a) {
   for (int tile = 0; tile < n; ++tile) {
     const int buffer = tile & 1;
     const R r = reader.at(buffer);
-    const int lane = threadIdx.x & 63;
     if (tile + 1 < n) load(0, tile + 1);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      f32x4 s[NK][2], dp[NK][2];
-      V8 p[NK], ds[NK];
+      f32x4 s[2], dp[2];
+      V8 p, ds;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int j = 0; j < NK; ++j) s[j][h] = 0.0f;
+        s[h] = 0.0f;
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) {
           const V8 f = R::template load<V8>((r.row ^ 64 * d) + (32 * t + 16 * h) * R::kRow);
-#pragma unroll
-          for (int j = 0; j < NK; ++j) s[j][h] = mfma16(f, k[j][d], s[j][h]);
+          s[h] = mfma16(f, k[d], s[h]);
         }
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const f32x4 from = *reinterpret_cast<const f32x4 *>(&stats[buffer][1][32 * t + 16 * h + 4 * (lane >> 4)]);   // dO v^T starts from -delta
-#pragma unroll
-        for (int j = 0; j < NK; ++j) dp[j][h] = from;
+        dp[h] = from;
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) {
           const V8 f = R::template load<V8>((r.row ^ 64 * d) + R::kBytes + (32 * t + 16 * h) * R::kRow);
-#pragma unroll
-          for (int j = 0; j < NK; ++j) dp[j][h] = mfma16(f, v[j][d], dp[j][h]);
+          dp[h] = mfma16(f, v[d], dp[h]);
         }
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const f32x4 l = *reinterpret_cast<const f32x4 *>(&stats[buffer][0][32 * t + 16 * h + 4 * (lane >> 4)]);
 #pragma unroll
-        for (int j = 0; j < NK; ++j) {
+        for (int r = 0; r < 4; ++r) s[h][r] = __builtin_amdgcn_exp2f(fmaf(s[h][r], a.c, -l[r]));
+        if (!all) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) s[j][h][r] = __builtin_amdgcn_exp2f(fmaf(s[j][h][r], a.c, -l[r]));
-          if (!all) {
+          for (int r = 0; r < 4; ++r) s[h][r] = on ? s[h][r] : 0.0f;
+        }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[j][h][r] = on[j] ? s[j][h][r] : 0.0f;
-          }
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            p[j][4 * h + r] = (T)s[j][h][r];
-            ds[j][4 * h + r] = (T)(s[j][h][r] * dp[j][h][r]);
-          }
+        for (int r = 0; r < 4; ++r) {
+          p[4 * h + r] = (T)s[h][r];
+          ds[4 * h + r] = (T)(s[h][r] * dp[h][r]);
         }
       }
 #pragma unroll
       for (int d = 0; d < DP / 16; ++d) {
         const V8 f = R::template load_columns<V8>((r.col ^ 32 * d) + R::kBytes + 32 * t * R::kRow, (r.col ^ 32 * d) + R::kBytes + (32 * t + 16) * R::kRow);
-#pragma unroll
-        for (int j = 0; j < NK; ++j) dv[j][d] = mfma16(f, p[j], dv[j][d]);
+        dv[d] = mfma16(f, p, dv[d]);
       }
 #pragma unroll
       for (int d = 0; d < DP / 16; ++d) {
         const V8 f = R::template load_columns<V8>((r.col ^ 32 * d) + 32 * t * R::kRow, (r.col ^ 32 * d) + (32 * t + 16) * R::kRow);
-#pragma unroll
-        for (int j = 0; j < NK; ++j) dk[j][d] = mfma16(f, ds[j], dk[j][d]);
+        dk[d] = mfma16(f, ds, dk[d]);
       }
       if (tile + 1 < n) {
         store(t, buffer ^ 1);
@@ -758,23 +742,19 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attend_dkv(AttArgs a) {
     }
     lds_barrier();
   }
+  if (!there) return;
+  const int64_t to = (((int64_t)b * a.Lk + key) * a.E + e) * a.D;
 #pragma unroll
-  for (int j = 0; j < NK; ++j) {
-    const int lane = threadIdx.x & 63, key = ((ct * WAVES + wave) * NK + j) * 16 + (lane & 15);
-    if (key >= a.Lk) continue;
-    const int64_t to = (((int64_t)b * a.Lk + key) * a.E + e) * a.D;
-#pragma unroll
-    for (int d = 0; d < DP / 16; ++d) {
-      const int at = 16 * d + 4 * (lane >> 4);
-      const float x[4] = {dk[j][d][0] * a.scale, dk[j][d][1] * a.scale, dk[j][d][2] * a.scale, dk[j][d][3] * a.scale};
-      const float y[4] = {dv[j][d][0], dv[j][d][1], dv[j][d][2], dv[j][d][3]};
-      store_n<4>((T *)a.dk + to + at, a.D - at, x);
-      store_n<4>((T *)a.dv + to + at, a.D - at, y);
-    }
+  for (int d = 0; d < DP / 16; ++d) {
+    const int at = 16 * d + 4 * (lane >> 4);
+    const float x[4] = {dk[d][0] * a.scale, dk[d][1] * a.scale, dk[d][2] * a.scale, dk[d][3] * a.scale};
+    const float y[4] = {dv[d][0], dv[d][1], dv[d][2], dv[d][3]};
+    store_n<4>((T *)a.dk + to + at, a.D - at, x);
+    store_n<4>((T *)a.dv + to + at, a.D - at, y);
   }
 }
 
-
+// Heads of 64 and less: a column of 32 keys a wave on v_mfma_f32_32x32x16, half the reads of LDS per product
 template <typename T, int DP, bool WHOLE>
 __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv32(AttArgs a) {
   typedef typename Vec<T>::type V8;
@@ -824,10 +804,10 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv32(AttArgs a) {
       });
     }
     if (which == 0 && threadIdx.x < kTile) {
-      const bool there = (int)threadIdx.x < left;
-      const int64_t row = be * a.rows + at + (there ? threadIdx.x : 0);
+      const bool in = (int)threadIdx.x < left;
+      const int64_t row = be * a.rows + at + (in ? threadIdx.x : 0);
       const float x = a.lse[row], y = a.delta[row];
-      lse = there ? x : INFINITY, delta = y;   // (behind the last row: probabilities of 0)
+      lse = in ? x : INFINITY, delta = y;   // (behind the last row: probabilities of 0)
     }
     if (WHOLE && which == 1 && (i0 += kTile) >= a.Lq) i0 = 0, ++g0;
   };
@@ -997,8 +977,8 @@ int launch_backward(AttArgs a, hipStream_t st) {
     if (whole) hipLaunchKernelGGL((k_attend_dkv32<T, DP, true>), g, blk, 0, st, a);
     else hipLaunchKernelGGL((k_attend_dkv32<T, DP, false>), g, blk, 0, st, a);
   } else {
-    if (whole) hipLaunchKernelGGL((k_attend_dkv<T, DP, 1, kWaves, true>), g, blk, 0, st, a);
-    else hipLaunchKernelGGL((k_attend_dkv<T, DP, 1, kWaves, false>), g, blk, 0, st, a);
+    if (whole) hipLaunchKernelGGL((k_attend_dkv16<T, DP, true>), g, blk, 0, st, a);
+    else hipLaunchKernelGGL((k_attend_dkv16<T, DP, false>), g, blk, 0, st, a);
   }
   return launched("k_attend_dkv");
 }

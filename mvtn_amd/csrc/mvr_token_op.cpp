@@ -236,7 +236,7 @@ Tensor attend_tokens(const Tensor &q, const Tensor &k, const Tensor &v, const Ma
                     "q, k and v share one type of float16, bfloat16");
   TORCH_CHECK_VALUE(in_32_bits(q) && in_32_bits(k), "every size of q, k and v must be below 2^31");
   const double scale = scale_.has_value() ? *scale_ : 1.0 / std::sqrt((double)D);
-  TORCH_CHECK_VALUE(scale > 0 && std::isfinite(scale), "scale must be positive and finite");
+  TORCH_CHECK_VALUE((float)scale > 0 && std::isfinite((float)scale), "scale must be positive and finite, in 32 bits too");
   Tensor keep = or_none(keep_);
   if (keep.defined()) {
     TORCH_CHECK_VALUE(keep.dim() == 2 && keep.size(0) == B && keep.size(1) >= 1 && Lk % keep.size(1) == 0, "keep is (B, G) with G a divisor of the ", Lk, " keys");

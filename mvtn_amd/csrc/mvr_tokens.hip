@@ -230,7 +230,7 @@ int launch_rotary(const RotArgs &a, int type, bool inter, bool bwd, mvr_stream_t
 //
 //   n = post N(branch)  (or branch),   y = residual + s g n,   z = N(y) weight + bias
 // N divides a row by the root of its mean square (+ eps), after taking its mean off for kind "layer".  A row lives in the registers of one
-// wave (up to 2048 wide forward, 1024 backward) or of a workgroup: one read, both norms' statistics by wave sums, one write.
+// wave or of several in a workgroup (norm_plan): one read, both norms' statistics by wave sums, one write.
 //
 // Backward, with r = 1 / std and hats for normed rows:
 //   dyt = dy + r_y (dz w - <dz w> - yhat <dz w yhat>)        (<>: mean over the row; the first mean only for "layer")

@@ -83,8 +83,9 @@ def attend_tokens(q, k, v, keep=None, scale=None):
     Hkv (consecutive heads share a key/value head); any strides whose last dimension is contiguous.  scale: D ** -0.5 by default.
 
     keep: (B, G) with G a divisor of Lk, non-zero where the Lk / G consecutive keys of a group stay — one entry per key, or one per view
-    (`draw_regularization`'s scale, viewed as (B, V)).  Keys that are left out are not read and get gradient 0; a query without any key
-    left gets 0.  Returns (B, Lq, H, D), differentiable with respect to q, k and v: the backward recomputes the probabilities."""
+    (`draw_regularization`'s scale, viewed as (B, V)).  Of keys that are left out nothing enters the output, whatever they hold, and they get
+    gradient 0; a query without any key left gets 0.  Returns (B, Lq, H, D), differentiable with respect to q, k and v: the backward recomputes
+    the probabilities."""
     return _lib.token_op().attend(q, k, v, keep, scale, _stream(q))
 
 
