@@ -3,10 +3,11 @@
 //   dV = P^T dO,  dS = P (dO v^T - delta),  delta = rowsum(dO O),  dQ = scale dS k,  dK = scale dS^T q
 // One pass over the keys with the running maximum and sum; nothing of size queries x keys is ever stored: the backward recomputes the
 // probabilities from q, k and lse.  Sums, maxima and exponentials are 32 bits wide; P and dS are rounded to the tensors' type where they
-// enter a matrix instruction: half a step of the type relative to each, as of the inputs.  (The forward's P lies in [0, 2^8], as its maximum may lag.)
+// enter a matrix instruction: half a step of the type relative to each, as of the inputs, and not where few keys make it count (FINE, at k_attend_dq).
+// The forward's P lies in [0, 2^8], as its maximum may lag.
 //
-// All three kernels have one shape.  A wave owns columns — queries (forward: two times 32 or 32, dQ: 32) or keys (dK/dV: 32 or 16) — and walks the other side in tiles that its
-// workgroup stages in LDS.  Scores come as tile x columns from v_mfma_f32_32x32x16: a lane then holds 16 scores of ONE column (rows 8 (r / 4) +
+// All three kernels have one shape.  A wave owns columns — queries (forward: 32 or two times 32, dQ: 32) or keys (dK/dV: 32 or 16) — and walks
+// the other side in tiles that its workgroup stages in LDS.  Scores come as tile x columns from v_mfma_f32_32x32x16: a lane then holds 16 scores of ONE column (rows 8 (r / 4) +
 // 4 (lane / 32) + r % 4), so softmax statistics need one exchange between the wave's halves, and eight consecutive registers are, with the
 // tile's rows taken in that same order, an operand of the next product: probabilities never leave the registers.  The other operand of
 // that product is the tile's transpose, which ds_read_b64_tr_b16 reads from the row-major tile.
@@ -225,6 +226,14 @@ __device__ __forceinline__ typename Vec<T>::type to_frag(const f32x16 &x, int ha
   for (int k = 0; k < 8; ++k) v[k] = (T)x[8 * half + k];
   return v;
 }
+// what to_frag's rounding leaves
+template <typename T>
+__device__ __forceinline__ typename Vec<T>::type rest_frag(const f32x16 &x, int half) {
+  typename Vec<T>::type v;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = (T)(x[8 * half + k] - (float)(T)x[8 * half + k]);
+  return v;
+}
 // x + the sum of an operand's eight values
 __device__ __forceinline__ float add_frag(bf16x8 p, float x) {
   typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -387,9 +396,15 @@ __device__ __forceinline__ void mask_scores(f32x16 &s, unsigned long long m, int
 // (Following every new maximum, one of a wave's 64 columns has one in four tiles of five, at 68 multiplications each.)
 constexpr float kSlack = 8.0f;
 
+// FINE (here and in the backward), where all keys lie in one tile: P and dS enter their products, and P the sum, as two parts, a rounded value and what
+// its rounding left, and delta comes from P and dP in 32 bits.  Otherwise the gradients carry, beside the store's rounding, one of P and dS (1.4
+// times the store's error alone, at any length), and that of the sum and of the stored output in delta, which average out over many keys
+// but not over few (1.6 times with 12 keys and heads of 64; 1.0 with FINE).  It costs, forward / backward: 384 x 64 tokens, 12 heads of 64 on 4
+// 30.4 -> 31.6 / 76 -> 87 us; 16 heads of 128 107 -> 109 / 292 us both; 64 x 1000 queries over 48 keys 60.7 -> 65 / 164 -> 179 us.
+//
 // NS columns of 32 queries a wave: with two, every operand read from LDS serves two products, and one's exponentials run beside the other's
 // products
-template <typename T, int DP, int NS, bool SPLIT, bool WHOLE>
+template <typename T, int DP, int NS, bool SPLIT, bool WHOLE, bool FINE>
 __global__ __launch_bounds__(kBlock, 2) void k_attend(AttArgs a) {
   typedef typename Vec<T>::type V8;
   constexpr int kSize = Layout<DP>::kSize;
@@ -435,6 +450,14 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend(AttArgs a) {
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int d = 0; d < DP / 32; ++d) o[n][d] = mfma(v[h][d], p[n][h], o[n][d]);
+          if constexpr (FINE) {
+            const V8 rest[2] = {rest_frag<T>(s[n][t], 0), rest_frag<T>(s[n][t], 1)};
+            sum[n] = add_frag(rest[1], add_frag(rest[0], sum[n]));
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int d = 0; d < DP / 32; ++d) o[n][d] = mfma(v[h][d], rest[h], o[n][d]);
+          }
         }
       }
       return;
@@ -525,7 +548,7 @@ __global__ __launch_bounds__(kBlock) void k_attend_join(AttArgs a) {
 // One column of 32 queries a wave: with heads of 64 160 registers and three waves a SIMD, where two columns take 246 and leave two.
 // 16 x 2352 tokens, 12 heads of 64, 12 views of which a quarter is dropped, bfloat16: 424 us against 472 with two; the forward, which keeps less
 // per column, takes 364 us with two and 411 with one.
-template <typename T, int DP, bool SPLIT, bool WHOLE>
+template <typename T, int DP, bool SPLIT, bool WHOLE, bool FINE>
 __global__ __launch_bounds__(kBlock, 2) void k_attend_dq(AttArgs a) {
   typedef typename Vec<T>::type V8;
   constexpr int kSize = Layout<DP>::kSize;
@@ -544,15 +567,18 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dq(AttArgs a) {
   float lse, delta = 0.0f;
   load_frags<T, DP>((const T *)a.q + b * a.qs[0] + c.i * a.qs[1] + h * a.qs[2], a, q);
   load_frags<T, DP>((const T *)a.go + b * a.gs[0] + c.i * a.gs[1] + h * a.gs[2], a, go);
-  V8 o[DP / 16];
-  load_frags<T, DP>((const T *)a.o + (((int64_t)b * a.Lq + c.i) * a.H + h) * a.D, a, o);
+  if constexpr (!FINE) {
+    V8 o[DP / 16];
+    load_frags<T, DP>((const T *)a.o + (((int64_t)b * a.Lq + c.i) * a.H + h) * a.D, a, o);
 #pragma unroll
-  for (int s = 0; s < DP / 16; ++s)
+    for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
-    for (int k = 0; k < 8; ++k) delta += (float)o[s][k] * (float)go[s][k];
-  delta += other_half(delta);
+      for (int k = 0; k < 8; ++k) delta += (float)o[s][k] * (float)go[s][k];
+    delta += other_half(delta);
+  }
   lse = c.live ? a.lse[be * a.rows + c.row] : INFINITY;
-  if (c.live && (threadIdx.x & 32) == 0 && split == 0) a.delta[be * a.rows + c.row] = delta;
+  const bool writes = c.live && (threadIdx.x & 32) == 0 && split == 0;
+  if (!FINE && writes) a.delta[be * a.rows + c.row] = delta;
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d) dq[d] = 0.0f;
   const T *kb = (const T *)a.k + b * a.ks[0] + e * a.ks[2], *vb = (const T *)a.v + b * a.vs[0] + e * a.vs[2];
@@ -562,6 +588,28 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dq(AttArgs a) {
   const auto step = [&](int buffer, unsigned long long m, int t) {
     const Reader<DP> r = reader.at(buffer);
     V8 f[DP / 16], kc[2][DP / 32];
+    if (FINE && t == 0) {   // delta over the one tile
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        f32x16 s = 0.0f, dp = 0.0f;
+        row_frags<T, DP>(r, 0, u, f);
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d) s = mfma(f[d], q[d], s);
+        fence();
+        row_frags<T, DP>(r, 1, u, f);
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d) dp = mfma(f[d], go[d], dp);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse));
+        if (m != ~0ull) mask_scores(s, m, u, 0.0f);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) delta = fmaf(s[r], dp[r], delta);
+        fence();
+      }
+      delta += other_half(delta);
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) dq[d] = 0.0f;   // (the zeros from before need no registers until here)
+    }
     f32x16 s = 0.0f, dp = 0.0f;
     row_frags<T, DP>(r, 0, t, f);
 #pragma unroll
@@ -578,6 +626,8 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dq(AttArgs a) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] *= dp[r] - delta;
     const V8 ds[2] = {to_frag<T>(s, 0), to_frag<T>(s, 1)};
+    V8 rest[2];
+    if constexpr (FINE) rest[0] = rest_frag<T>(s, 0), rest[1] = rest_frag<T>(s, 1);
     if (DP > 64) {   // (the scores have been used up: their registers take the operands)
       fence();
       col_frags<T, DP>(r, 0, t, kc);
@@ -585,10 +635,14 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dq(AttArgs a) {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int d = 0; d < DP / 32; ++d) dq[d] = mfma(kc[h][d], ds[h], dq[d]);
+      for (int d = 0; d < DP / 32; ++d) {
+        dq[d] = mfma(kc[h][d], ds[h], dq[d]);
+        if constexpr (FINE) dq[d] = mfma(kc[h][d], rest[h], dq[d]);
+      }
     fence();
   };
   walk_tiles(a, b, first, last, MVR_ATT_KV, step);
+  if (FINE && writes) a.delta[be * a.rows + c.row] = delta;
   if (c.live) {
     if constexpr (SPLIT) store_column<float, DP>(a.part + ((split * (int64_t)a.B * a.E + be) * a.rows + c.row) * a.D, a.D, dq, 1.0f);
     else store_column<T, DP>((T *)a.dq + (((int64_t)b * a.Lq + c.i) * a.H + e * a.G + c.g) * a.D, a.D, dq, a.scale);
@@ -616,7 +670,7 @@ __global__ __launch_bounds__(kBlock) void k_attend_dq_join(AttArgs a) {
 // keys of 128 fill all of one.  A lane's scores are rows 16 b + 4 (lane / 16) + 0..3 of a sub-tile of 32 (b = 0, 1) of ONE key, which is the order
 // that the next product's operands take the rows in.
 
-template <typename T, int DP, bool WHOLE>
+template <typename T, int DP, bool WHOLE, bool FINE>
 __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv16(AttArgs a) {
   typedef typename Vec<T>::type V8;
   typedef Reader<DP> R;
@@ -690,7 +744,7 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv16(AttArgs a) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       f32x4 s[2], dp[2];
-      V8 p, ds;
+      V8 p, ds, p_rest, ds_rest;   // (the rests with FINE alone)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         s[h] = 0.0f;
@@ -723,17 +777,23 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv16(AttArgs a) {
         for (int r = 0; r < 4; ++r) {
           p[4 * h + r] = (T)s[h][r];
           ds[4 * h + r] = (T)(s[h][r] * dp[h][r]);
+          if constexpr (FINE) {
+            p_rest[4 * h + r] = (T)(s[h][r] - (float)p[4 * h + r]);
+            ds_rest[4 * h + r] = (T)(s[h][r] * dp[h][r] - (float)ds[4 * h + r]);
+          }
         }
       }
 #pragma unroll
       for (int d = 0; d < DP / 16; ++d) {
         const V8 f = R::template load_columns<V8>((r.col ^ 32 * d) + R::kBytes + 32 * t * R::kRow, (r.col ^ 32 * d) + R::kBytes + (32 * t + 16) * R::kRow);
         dv[d] = mfma16(f, p, dv[d]);
+        if constexpr (FINE) dv[d] = mfma16(f, p_rest, dv[d]);
       }
 #pragma unroll
       for (int d = 0; d < DP / 16; ++d) {
         const V8 f = R::template load_columns<V8>((r.col ^ 32 * d) + 32 * t * R::kRow, (r.col ^ 32 * d) + (32 * t + 16) * R::kRow);
         dk[d] = mfma16(f, ds, dk[d]);
+        if constexpr (FINE) dk[d] = mfma16(f, ds_rest, dk[d]);
       }
       if (tile + 1 < n) {
         store(t, buffer ^ 1);
@@ -755,7 +815,7 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv16(AttArgs a) {
 }
 
 // Heads of 64 and less: a column of 32 keys a wave on v_mfma_f32_32x32x16, half the reads of LDS per product
-template <typename T, int DP, bool WHOLE>
+template <typename T, int DP, bool WHOLE, bool FINE>
 __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv32(AttArgs a) {
   typedef typename Vec<T>::type V8;
   constexpr int kSize = Layout<DP>::kSize;
@@ -860,7 +920,10 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv32(AttArgs a) {
 #pragma unroll
       for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d) dv[d] = mfma(c[half][d], p[half], dv[d]);
+        for (int d = 0; d < DP / 32; ++d) {
+          dv[d] = mfma(c[half][d], p[half], dv[d]);
+          if constexpr (FINE) dv[d] = mfma(c[half][d], rest_frag<T>(s, half), dv[d]);
+        }
       dp *= s;
       const V8 ds[2] = {to_frag<T>(dp, 0), to_frag<T>(dp, 1)};
       fence();
@@ -868,7 +931,10 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv32(AttArgs a) {
 #pragma unroll
       for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d) dk[d] = mfma(c2[half][d], ds[half], dk[d]);
+        for (int d = 0; d < DP / 32; ++d) {
+          dk[d] = mfma(c2[half][d], ds[half], dk[d]);
+          if constexpr (FINE) dk[d] = mfma(c2[half][d], rest_frag<T>(dp, half), dk[d]);
+        }
       fence();
       if (tile + 1 < n) {
         store(t, buffer ^ 1);
@@ -938,15 +1004,21 @@ int launch_forward(AttArgs a, hipStream_t st) {
   if (!grid_of(a, a.rows, 32 * kWaves * (1 + a.wide), a.splits, n)) return bad("mvr_attend_tokens_forward: too many workgroups");
   const dim3 g(n), blk(kBlock);
   constexpr int kWide = DP <= 64 ? 2 : 1;
-  if (a.splits == 1) {
-    if (a.wide) hipLaunchKernelGGL((k_attend<T, DP, kWide, false, true>), g, blk, 0, st, a);
-    else if (a.whole) hipLaunchKernelGGL((k_attend<T, DP, 1, false, true>), g, blk, 0, st, a);
-    else hipLaunchKernelGGL((k_attend<T, DP, 1, false, false>), g, blk, 0, st, a);
+  if (a.tiles == 1) {
+    if (a.wide) hipLaunchKernelGGL((k_attend<T, DP, kWide, false, true, true>), g, blk, 0, st, a);
+    else if (a.whole) hipLaunchKernelGGL((k_attend<T, DP, 1, false, true, true>), g, blk, 0, st, a);
+    else hipLaunchKernelGGL((k_attend<T, DP, 1, false, false, true>), g, blk, 0, st, a);
     return launched("k_attend");
   }
-  if (a.wide) hipLaunchKernelGGL((k_attend<T, DP, kWide, true, true>), g, blk, 0, st, a);
-  else if (a.whole) hipLaunchKernelGGL((k_attend<T, DP, 1, true, true>), g, blk, 0, st, a);
-  else hipLaunchKernelGGL((k_attend<T, DP, 1, true, false>), g, blk, 0, st, a);
+  if (a.splits == 1) {
+    if (a.wide) hipLaunchKernelGGL((k_attend<T, DP, kWide, false, true, false>), g, blk, 0, st, a);
+    else if (a.whole) hipLaunchKernelGGL((k_attend<T, DP, 1, false, true, false>), g, blk, 0, st, a);
+    else hipLaunchKernelGGL((k_attend<T, DP, 1, false, false, false>), g, blk, 0, st, a);
+    return launched("k_attend");
+  }
+  if (a.wide) hipLaunchKernelGGL((k_attend<T, DP, kWide, true, true, false>), g, blk, 0, st, a);
+  else if (a.whole) hipLaunchKernelGGL((k_attend<T, DP, 1, true, true, false>), g, blk, 0, st, a);
+  else hipLaunchKernelGGL((k_attend<T, DP, 1, true, false, false>), g, blk, 0, st, a);
   if (int rc = launched("k_attend")) return rc;
   hipLaunchKernelGGL((k_attend_join<T>), dim3((unsigned)((lines(a) + kWaves - 1) / kWaves)), dim3(kBlock), 0, st, a);
   return launched("k_attend_join");
@@ -956,12 +1028,16 @@ template <typename T, int DP>
 int launch_backward(AttArgs a, hipStream_t st) {
   unsigned n;
   if (!grid_of(a, a.rows, 32 * kWaves, a.splits, n)) return bad("mvr_attend_tokens_backward: too many workgroups");
-  if (a.splits == 1) {
-    if (a.whole) hipLaunchKernelGGL((k_attend_dq<T, DP, false, true>), dim3(n), dim3(kBlock), 0, st, a);
-    else hipLaunchKernelGGL((k_attend_dq<T, DP, false, false>), dim3(n), dim3(kBlock), 0, st, a);
+  const bool fine = a.tiles == 1;
+  if (fine) {
+    if (a.whole) hipLaunchKernelGGL((k_attend_dq<T, DP, false, true, true>), dim3(n), dim3(kBlock), 0, st, a);
+    else hipLaunchKernelGGL((k_attend_dq<T, DP, false, false, true>), dim3(n), dim3(kBlock), 0, st, a);
+  } else if (a.splits == 1) {
+    if (a.whole) hipLaunchKernelGGL((k_attend_dq<T, DP, false, true, false>), dim3(n), dim3(kBlock), 0, st, a);
+    else hipLaunchKernelGGL((k_attend_dq<T, DP, false, false, false>), dim3(n), dim3(kBlock), 0, st, a);
   } else {
-    if (a.whole) hipLaunchKernelGGL((k_attend_dq<T, DP, true, true>), dim3(n), dim3(kBlock), 0, st, a);
-    else hipLaunchKernelGGL((k_attend_dq<T, DP, true, false>), dim3(n), dim3(kBlock), 0, st, a);
+    if (a.whole) hipLaunchKernelGGL((k_attend_dq<T, DP, true, true, false>), dim3(n), dim3(kBlock), 0, st, a);
+    else hipLaunchKernelGGL((k_attend_dq<T, DP, true, false, false>), dim3(n), dim3(kBlock), 0, st, a);
   }
   if (int rc = launched("k_attend_dq")) return rc;
   if (a.splits > 1) {
@@ -973,13 +1049,16 @@ int launch_backward(AttArgs a, hipStream_t st) {
   constexpr int kKeys = DP <= 64 ? 32 * kWaves : 16 * kWaves;
   if (!grid_of(a, a.Lk, kKeys, 1, n)) return bad("mvr_attend_tokens_backward: too many workgroups");
   const dim3 g(n), blk(kBlock);
-  if constexpr (DP <= 64) {
-    if (whole) hipLaunchKernelGGL((k_attend_dkv32<T, DP, true>), g, blk, 0, st, a);
-    else hipLaunchKernelGGL((k_attend_dkv32<T, DP, false>), g, blk, 0, st, a);
-  } else {
-    if (whole) hipLaunchKernelGGL((k_attend_dkv16<T, DP, true>), g, blk, 0, st, a);
-    else hipLaunchKernelGGL((k_attend_dkv16<T, DP, false>), g, blk, 0, st, a);
-  }
+#define MVR_ATT_KEYS(kernel)                                                                \
+  do {                                                                                      \
+    if (fine && whole) hipLaunchKernelGGL((kernel<T, DP, true, true>), g, blk, 0, st, a);   \
+    else if (fine) hipLaunchKernelGGL((kernel<T, DP, false, true>), g, blk, 0, st, a);      \
+    else if (whole) hipLaunchKernelGGL((kernel<T, DP, true, false>), g, blk, 0, st, a);     \
+    else hipLaunchKernelGGL((kernel<T, DP, false, false>), g, blk, 0, st, a);               \
+  } while (0)
+  if constexpr (DP <= 64) MVR_ATT_KEYS(k_attend_dkv32);
+  else MVR_ATT_KEYS(k_attend_dkv16);
+#undef MVR_ATT_KEYS
   return launched("k_attend_dkv");
 }
 

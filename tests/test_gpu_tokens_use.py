@@ -38,6 +38,23 @@ def test_more_shapes_match_the_definition(dtype, B, Lq, Lk, H, E, D, groups, dro
     _matches_the_definition(dtype, B, Lq, Lk, H, E, D, groups, dropped)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Lq,Lk,H,E,D,groups", [(13, 36, 6, 2, 40, 12), (12, 12, 4, 4, 64, 0), (70, 64, 4, 2, 128, 8), (200, 20, 2, 2, 32, 5), (1, 7, 4, 1, 96, 0), (9, 33, 2, 1, 125, 0)])
+def test_gradients_over_few_keys_carry_one_rounding(dtype, Lq, Lk, H, E, D, groups):
+    """Where all keys lie in one tile P and dS are not rounded to 16 bits: a gradient carries its store's rounding u, what two 16-bit parts leave of P
+    and dS (u^2 relative; below 2^-14 of float16 at most 2^-25 each), and 32-bit arithmetic, all against the absolute sums."""
+    g = _gen(52)
+    q, k, v, do = (_randn(g, *s, dtype=dtype) for s in ((2, Lq, H, D), (2, Lk, E, D), (2, Lk, E, D), (2, Lq, H, D)))
+    keep = torch.rand(2, groups, generator=g, device=_dev()) < 0.5 if groups else None
+    got = _all(q, k, v, do, keep=keep)
+    want, size = _attend64(q, k, v, keep, D ** -0.5, do)
+    u = _u(dtype)
+    small = 2 * u * u + 2.0 ** -24 * (4 * D + 64)
+    low = 2.0 ** -25 * (6 * max(Lk, Lq * (H // E)) + 1) if dtype == torch.float16 else 0.0
+    for name, a, w, s in zip(("dq", "dk", "dv"), got[1:], want[1:], size[1:]):
+        assert ((a.double() - w).abs() <= u * w.abs() + 2 * small * s + low + 1e-30).all(), name
+
+
 def _unaligned(t):
     """The same values, one element behind an aligned address."""
     return torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)[1:].view(t.shape).copy_(t)
