@@ -460,14 +460,15 @@ typedef struct mvr_norm_params {
 } mvr_norm_params;
 
 /* All tensors contiguous.  A row whose `scale` is 0 (a dropped view) keeps its residual; its branch is not read.
- * stats: (rows, 4) f32 for the backward, or NULL.  y may be residual itself. */
+ * stats: (rows, 4) f32 for the backward, or NULL.  y may be residual itself, where no backward follows or the residual has 32 bits. */
 int mvr_add_norm_tokens_forward(const mvr_norm_params *params, const void *residual, const void *branch, const void *weight,
                                 const void *bias, const void *post_weight, const void *gate, const float *scale, void *y,
                                 void *z, float *stats, mvr_stream_t stream);
 size_t mvr_add_norm_tokens_workspace_bytes(const mvr_norm_params *params);
-/* grad_y or grad_z may be NULL (zero), the parameters' gradients may each be NULL (not wanted).  The workspace is needed for
+/* y_or_residual: the forward's y where the residual has 32 bits, its residual where it has 16 (y is formed again, without its rounding).
+ * grad_y or grad_z may be NULL (zero), the parameters' gradients may each be NULL (not wanted).  The workspace is needed for
  * the latter; sums are taken in a fixed order (bit-reproducible). */
-int mvr_add_norm_tokens_backward(const mvr_norm_params *params, const void *y, const void *branch, const void *weight,
+int mvr_add_norm_tokens_backward(const mvr_norm_params *params, const void *y_or_residual, const void *branch, const void *weight,
                                  const void *post_weight, const void *gate, const float *scale, const float *stats,
                                  const void *grad_y, const void *grad_z, void *grad_residual, void *grad_branch,
                                  void *grad_weight, void *grad_bias, void *grad_post_weight, void *grad_gate,

@@ -276,7 +276,8 @@ struct AddNorm : public torch::autograd::Function<AddNorm> {
     Tensor y, z;
     const Tensor stats = norm_forward(p, t, y, z, true, stream);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({y, t.branch, t.weight, t.post, t.gate, draws, stats});
+    // (y in 32 bits is what the backward needs; in 16 bits it would bring its rounding along, and the backward forms it again)
+    ctx->save_for_backward({p.residual_type == MVR_TYPE_FLOAT ? y : t.residual, t.branch, t.weight, t.post, t.gate, draws, stats});
     ctx->saved_data["params"] = params;
     ctx->saved_data["stream"] = stream;
     ctx->saved_data["need"] = std::vector<int64_t>{weight.requires_grad(), bias.defined() && bias.requires_grad(), post.defined() && post.requires_grad(),
@@ -287,7 +288,7 @@ struct AddNorm : public torch::autograd::Function<AddNorm> {
     variable_list none(9);
     if (!grads[0].defined() && !grads[1].defined()) return none;
     const auto s = ctx->get_saved_variables();
-    const Tensor &y = s[0], &branch = s[1], &weight = s[2], &post = s[3], &gate = s[4], &draws = s[5], &stats = s[6];
+    const Tensor &y = s[0] /* or the residual */, &branch = s[1], &weight = s[2], &post = s[3], &gate = s[4], &draws = s[5], &stats = s[6];
     const auto need = ctx->saved_data["need"].toIntVector();
     mvr_norm_params p;
     std::memcpy(&p, ctx->saved_data["params"].toStringRef().data(), sizeof(p));

@@ -236,14 +236,16 @@ int launch_rotary(const RotArgs &a, int type, bool inter, bool bwd, mvr_stream_t
 //   dyt = dy + r_y (dz w - <dz w> - yhat <dz w yhat>)        (<>: mean over the row; the first mean only for "layer")
 //   dresidual = dyt,  dn = s g dyt,  dbranch = r_a (dn post - <dn post> - ahat <dn post ahat>)
 // and the column sums dweight = sum dz yhat, dbias = sum dz, dpost = sum dn ahat, dgate = sum s post ahat dyt.  A workgroup sums the columns
-// of its rows in registers and leaves one line of partial sums; k_norm_columns adds the lines up in a fixed order.
+// of its rows in registers and leaves one line of partial sums; k_norm_columns adds the lines up in a fixed order.  y is had again from the residual
+// and the branch where its stored form has 16 bits: yhat and everything that follows would carry its rounding (1.4 times the error of dweight's
+// own store); with 32 bits it is read as stored.  Either way the same number of bytes (16 x 2352 x 768 bf16: 82 us, 79 from the stored y).
 
 struct NormArgs {
   const void *residual, *branch, *weight, *bias, *post, *gate;
   const float *scale;
   void *y, *z;
   float *stats;             // (rows, 4): mean and 1 / std of y, of branch
-  // backward: residual = y as stored, dy / dz either may be null
+  // backward: residual = y as stored where it has 32 bits, the residual itself where it has 16; dy / dz either may be null
   const void *dy, *dz;
   void *dresidual, *dbranch;
   float *partial;           // (blocks, 4, D): dweight, dbias, dpost, dgate
@@ -450,6 +452,14 @@ __global__ __launch_bounds__(WAVES > 1 ? 64 * WAVES : kBlock) void k_add_norm_ba
       const float4 w4 = params[j * kLanes + lane][0];
       const float w[kV] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
+      for (int k = 0; k < kV; ++k) n[j][k] = gone || k >= left[j] ? 0.0f : a.post ? (n[j][k] - st.z) * st.w : n[j][k];   // ahat (or the branch)
+      if constexpr (sizeof(TR) == 2) {   // y from the residual
+        const float4 p4 = params[j * kLanes + lane][1], g4 = params[j * kLanes + lane][2];
+        const float po[kV] = {p4.x, p4.y, p4.z, p4.w}, ga[kV] = {g4.x, g4.y, g4.z, g4.w};
+#pragma unroll
+        for (int k = 0; k < kV; ++k) y[j][k] += gone ? 0.0f : s0 * (n[j][k] * po[k] * ga[k]);
+      }
+#pragma unroll
       for (int k = 0; k < kV; ++k) {
         y[j][k] = k < left[j] ? (y[j][k] - st.x) * st.y : 0.0f;   // yhat
         dw[j][k] += g[j][k] * y[j][k];
@@ -469,12 +479,11 @@ __global__ __launch_bounds__(WAVES > 1 ? 64 * WAVES : kBlock) void k_add_norm_ba
 #pragma unroll
       for (int k = 0; k < kV; ++k) {
         t[j][k] += st.y * (g[j][k] - m1 - y[j][k] * m0);          // dyt
-        const float hat = gone || k >= left[j] ? 0.0f : a.post ? (n[j][k] - st.z) * st.w : n[j][k];
+        const float hat = n[j][k];
         const float u = k < left[j] ? s0 * t[j][k] : 0.0f;
         dg[j][k] += u * po[k] * hat;
         const float dn = gone ? 0.0f : u * ga[k];
         dp[j][k] += dn * hat;
-        n[j][k] = hat;
         g[j][k] = dn * po[k];
         d[0] += g[j][k] * hat;
         d[1] += g[j][k];
@@ -562,11 +571,11 @@ int norm_args(NormArgs &a, const mvr_norm_params *p) {
   return MVR_OK;
 }
 
-// 256 elements of a row per wave and vector.  Rows of up to 768 lie in one wave's registers (16 x 2352 x 768 bf16, forward / backward: 55.5 / 78.6 us;
-// a row over the three waves of a workgroup: 69 / 82 with its columns); wider ones take a workgroup: 64 x 3920 x 1024 forward 586 us, with one
+// 256 elements of a row per wave and vector.  Rows of up to 768 lie in one wave's registers (16 x 2352 x 768 bf16, forward / backward: 55.5 / 82 us;
+// a row over the three waves of a workgroup, measured where the backward above took 78.6: 69 / 82 with its columns); wider ones take a workgroup: 64 x 3920 x 1024 forward 586 us, with one
 // wave a row 622.
 // Grids hold as many workgroups as are resident at once (256 CUs by what the registers allow) and every wave runs through its rows: a second,
-// partly filled round costs more than it balances (backward at 768: 512 workgroups 79 us, 768 101, 1024 87).
+// partly filled round costs more than it balances (backward at 768, before y was formed again: 512 workgroups 79 us, 768 101, 1024 87).
 struct NormPlan { int32_t waves, vectors, forward, backward; };
 inline NormPlan norm_plan(int32_t D) {
   return D <= 256 ? NormPlan{1, 1, 2048, 1280} : D <= 512 ? NormPlan{1, 2, 1280, 768} : D <= 768 ? NormPlan{1, 3, 1024, 512}
@@ -675,7 +684,7 @@ extern "C" int mvr_add_norm_tokens_backward(const mvr_norm_params *params, const
   NormArgs a = {};
   if (int rc = norm_args(a, params)) return rc;
   if (!y || !branch || !weight || !stats || (!grad_y && !grad_z) || !grad_residual || !grad_branch)
-    return bad("mvr_add_norm_tokens_backward: y, branch, weight, stats, one of grad_y and grad_z, grad_residual and grad_branch must be given");
+    return bad("mvr_add_norm_tokens_backward: y_or_residual, branch, weight, stats, one of grad_y and grad_z, grad_residual and grad_branch must be given");
   if ((gate != nullptr) != (params->gate_groups > 0) || (scale != nullptr) != (params->scale_groups > 0))
     return bad("mvr_add_norm_tokens_backward: gate and scale go with their groups");
   if ((grad_gate && !gate) || (grad_post_weight && !post_weight)) return bad("mvr_add_norm_tokens_backward: a gradient of a parameter that is not there");

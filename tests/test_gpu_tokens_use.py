@@ -9,7 +9,7 @@ from mvtn_amd import tokens
 from mvtn_amd.regularize import draw_regularization
 
 from gpu_helpers import _dev
-from test_gpu_tokens import _attend64, _gen, _randn, _rotary64, _u
+from test_gpu_tokens import U32, _attend64, _gen, _norm64, _randn, _rotary64, _tiny, _u
 from test_gpu_tokens import test_attention_matches_the_definition as _matches_the_definition
 
 pytestmark = pytest.mark.gpu
@@ -53,6 +53,31 @@ def test_gradients_over_few_keys_carry_one_rounding(dtype, Lq, Lk, H, E, D, grou
     low = 2.0 ** -25 * (6 * max(Lk, Lq * (H // E)) + 1) if dtype == torch.float16 else 0.0
     for name, a, w, s in zip(("dq", "dk", "dv"), got[1:], want[1:], size[1:]):
         assert ((a.double() - w).abs() <= u * w.abs() + 2 * small * s + low + 1e-30).all(), name
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kind,post,gate,views,D", [("rms", False, None, 0, 384), ("rms", False, "channel", 4, 384), ("layer", True, "object", 4, 837), ("rms", True, "channel", 0, 1500)])
+def test_norm_gradients_of_16_bit_streams_carry_one_rounding(dtype, kind, post, gate, views, D):
+    """y's rounding does not enter the backward: a gradient is off by its own store's u, relative to the tensor's 2-norm, and by 32-bit sums over D and
+    over the rows (100 2^-24, as for 32-bit streams)."""
+    g = _gen(D + 7)
+    B, L = 3, 20
+    t = {"residual": _randn(g, B, L, D, dtype=dtype) * 2, "branch": _randn(g, B, L, D, dtype=dtype), "weight": 1 + 0.2 * _randn(g, D, dtype=dtype),
+         "post": 1 + 0.2 * _randn(g, D, dtype=dtype) if post else None, "gate": None if gate is None else _randn(g, *((B, D) if gate == "object" else (D,)), dtype=dtype)}
+    draws = rows = None
+    if views:
+        draws = (torch.rand(B, views, generator=g, device=_dev()) >= 0.4).float() / 0.6
+        draws[0, 0] = 0.0
+        rows = draws.double().repeat_interleave(L // views, 1)[..., None]
+    leaves = {k: v.detach().requires_grad_() for k, v in t.items() if v is not None}
+    dy, dz = _randn(g, B, L, D, dtype=dtype), _randn(g, B, L, D, dtype=dtype)
+    out = tokens.add_norm_tokens(leaves["residual"], leaves["branch"], leaves["weight"], post_weight=leaves.get("post"), gate=leaves.get("gate"), scale=draws, kind=kind)
+    got = dict(zip(leaves, torch.autograd.grad(out, list(leaves.values()), (dy, dz))))
+    wy, wz, w = _norm64(t, kind, 1e-6, rows)
+    want = dict(zip(leaves, torch.autograd.grad((wy, wz), [w[k] for k in leaves], (dy.double(), dz.double()))))
+    for k, a in got.items():
+        far, norm = (a.double() - want[k]).norm(), want[k].norm()
+        assert far <= (_u(dtype) + 100 * U32) * norm + _tiny(dtype) * a.numel() ** 0.5, (k, float(far / norm))
 
 
 def _unaligned(t):
