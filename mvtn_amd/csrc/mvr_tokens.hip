@@ -572,8 +572,8 @@ int norm_args(NormArgs &a, const mvr_norm_params *p) {
 }
 
 // 256 elements of a row per wave and vector.  Rows of up to 768 lie in one wave's registers (16 x 2352 x 768 bf16, forward / backward: 55.5 / 82 us;
-// a row over the three waves of a workgroup, measured where the backward above took 78.6: 69 / 82 with its columns); wider ones take a workgroup: 64 x 3920 x 1024 forward 586 us, with one
-// wave a row 622.
+// a row over the three waves of a workgroup 69 / 82 with its columns, where the backward of one wave a row took 79); wider ones take a workgroup:
+// 64 x 3920 x 1024 forward 586 us, with one wave a row 622.
 // Grids hold as many workgroups as are resident at once (256 CUs by what the registers allow) and every wave runs through its rows: a second,
 // partly filled round costs more than it balances (backward at 768, before y was formed again: 512 workgroups 79 us, 768 101, 1024 87).
 struct NormPlan { int32_t waves, vectors, forward, backward; };
