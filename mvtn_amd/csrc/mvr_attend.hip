@@ -743,6 +743,7 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv16(AttArgs a) {
     if (tile + 1 < n) load(0, tile + 1);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
+      if (!WHOLE && t == 1 && a.rows - tile * kTile <= 32) break;   // the list's last tile: no rows in its second half (64 x 4 rows over 3920 keys of 128: 273 -> 262 us)
       f32x4 s[2], dp[2];
       V8 p, ds, p_rest, ds_rest;   // (the rests with FINE alone)
 #pragma unroll
@@ -892,6 +893,7 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv32(AttArgs a) {
     fence();
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
+      if (!WHOLE && t == 1 && a.rows - tile * kTile <= 32) break;   // the list's last tile: no rows in its second half
       f32x16 s = 0.0f, dp, l;
       row_frags<T, DP>(r, 1, t, gf);
 #pragma unroll
