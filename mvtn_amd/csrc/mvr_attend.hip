@@ -4,7 +4,8 @@
 // One pass over the keys with the running maximum and sum; nothing of size queries x keys is ever stored: the backward recomputes the
 // probabilities from q, k and lse.  Sums, maxima and exponentials are 32 bits wide; P and dS are rounded to the tensors' type where they
 // enter a matrix instruction: half a step of the type relative to each, as of the inputs, and not where few keys make it count (FINE, at k_attend_dq).
-// The forward's P lies in [0, 2^8], as its maximum may lag.
+// The forward's P lies in [0, 2^8], as its maximum may lag.  In float16, whose step stops shrinking at 2^-14, P and dS enter times a power of two
+// that brings them to the top of its range, and the 32-bit sums are divided by it (at kLift).
 //
 // All three kernels have one shape.  A wave owns columns — queries (forward: 32 or two times 32, dQ: 32) or keys (dK/dV: 32 or 16) — and walks
 // the other side in tiles that its workgroup stages in LDS.  Scores come as tile x columns from v_mfma_f32_32x32x16: a lane then holds 16 scores of ONE column (rows 8 (r / 4) +
@@ -253,6 +254,23 @@ __device__ __forceinline__ float add_frag(f16x8 p, float x) {
   for (int k = 0; k < 4; ++k) x = __builtin_amdgcn_fdot2(h[k], one, x, false);
   return x;
 }
+// Powers of two for float16.  A row's P over some thousand keys is about 2^-12 and dS = P (dP - delta) smaller still by what a loss' gradient is
+// below 1: rounded as they are, most would lie under 2^-14, where float16 keeps 2^-24 of anything (2352 keys, dO of 1e-3: dQ and dK off by 6 and 4 times
+// the store's own rounding; times these powers 1.1).
+// P: 2^kLift in the forward, where it reaches 2^kSlack without; 2^kLiftP in dK and dV, where it reaches 1.  Both come with the exponent, for nothing.
+// dS: one power per column (a query's in dQ, a key's in dK), the largest that keeps |dS| below kMost; like the running maximum it is found on the way:
+// it starts at 2^kStart, and where a value leaves the range all of the column so far is multiplied down until the largest is at kAim.  Powers of two: nothing
+// else is rounded.  bfloat16 has the exponents of 32 bits and needs none of it.
+// Forward and gradients of float16 with and without: 16 x 2352 tokens, 12 heads of 64, 1344 / 1296 us; 8 x 3920, 16 heads of 128, 5192 / 5106.
+template <typename T> constexpr bool kNarrow = false;
+template <> constexpr bool kNarrow<f16> = true;
+template <typename T> constexpr float kLift = kNarrow<T> ? 7.0f : 0.0f;
+template <typename T> constexpr float kLiftP = kNarrow<T> ? 14.0f : 0.0f;
+constexpr float kStart = 60.0f, kMost = 32768.0f;
+constexpr int kAim = 8;
+__device__ __forceinline__ float power_of_2(int n) { return __builtin_bit_cast(float, (unsigned)(127 + n) << 23); }
+__device__ __forceinline__ int exponent_of(float x) { return (int)(__builtin_bit_cast(unsigned, x) >> 23) - 127; }   // x >= 0; 128 for infinity
+
 // Waits for every load issued so far.  Called in front of a loop that keeps loads in flight: a register loaded before the loop would otherwise
 // be waited for inside it, and the wait for it is a wait for everything.
 __device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0F70); }   // vmcnt(0)
@@ -441,7 +459,7 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend(AttArgs a) {
         col_frags<T, DP>(r, 1, t, v);
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
-          const float off = top[n] == -INFINITY ? 0.0f : top[n];
+          const float off = top[n] == -INFINITY ? 0.0f : top[n] - kLift<T>;
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[n][t][r] = __builtin_amdgcn_exp2f(fmaf(s[n][t][r], a.c, -off));
           p[n][0] = to_frag<T>(s[n][t], 0), p[n][1] = to_frag<T>(s[n][t], 1);
@@ -511,10 +529,10 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend(AttArgs a) {
     if constexpr (SPLIT) {
       const int64_t line = (split * (int64_t)a.B * a.E + be) * a.rows + c.row;
       store_column<float, DP>(a.part + line * a.D, a.D, o[n], inv);
-      if (hi == 0) a.part_lse[line] = all == 0.0f ? -INFINITY : top[n] + __builtin_amdgcn_logf(all);
+      if (hi == 0) a.part_lse[line] = all == 0.0f ? -INFINITY : top[n] - kLift<T> + __builtin_amdgcn_logf(all);
     } else {
       store_column<T, DP>((T *)a.out + (((int64_t)b * a.Lq + c.i) * a.H + e * a.G + c.g) * a.D, a.D, o[n], inv);
-      if (a.lse && hi == 0) a.lse[be * a.rows + c.row] = all == 0.0f ? INFINITY : top[n] + __builtin_amdgcn_logf(all);
+      if (a.lse && hi == 0) a.lse[be * a.rows + c.row] = all == 0.0f ? INFINITY : top[n] - kLift<T> + __builtin_amdgcn_logf(all);
     }
   }
 }
@@ -565,6 +583,7 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dq(AttArgs a) {
   const Column c = column_of(a, ct, 0, 32);
   const int h = e * a.G + c.g;
   float lse, delta = 0.0f;
+  float power = kNarrow<T> ? kStart : 0.0f;   // log2 of what this column's dS and dq are multiplied by (it goes into P's exponent)
   load_frags<T, DP>((const T *)a.q + b * a.qs[0] + c.i * a.qs[1] + h * a.qs[2], a, q);
   load_frags<T, DP>((const T *)a.go + b * a.gs[0] + c.i * a.gs[1] + h * a.gs[2], a, go);
   if constexpr (!FINE) {
@@ -621,10 +640,24 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dq(AttArgs a) {
     fence();
     if (DP <= 64) col_frags<T, DP>(r, 0, t, kc);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -lse));
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, kNarrow<T> ? power - lse : -lse));
     if (m != ~0ull) mask_scores(s, m, t, 0.0f);
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] *= dp[r] - delta;
+    if constexpr (kNarrow<T>) {
+      float most = 0.0f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(s[r]));
+      if (__any(most > kMost)) {
+        most = fmaxf(most, other_half(most));
+        const int down = most > kMost ? exponent_of(most) - kAim : 0;
+        const float by = power_of_2(-down);
+        s *= by;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) dq[d] *= by;
+        power -= (float)down;
+      }
+    }
     const V8 ds[2] = {to_frag<T>(s, 0), to_frag<T>(s, 1)};
     V8 rest[2];
     if constexpr (FINE) rest[0] = rest_frag<T>(s, 0), rest[1] = rest_frag<T>(s, 1);
@@ -644,8 +677,9 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dq(AttArgs a) {
   walk_tiles(a, b, first, last, MVR_ATT_KV, step);
   if (FINE && writes) a.delta[be * a.rows + c.row] = delta;
   if (c.live) {
-    if constexpr (SPLIT) store_column<float, DP>(a.part + ((split * (int64_t)a.B * a.E + be) * a.rows + c.row) * a.D, a.D, dq, 1.0f);
-    else store_column<T, DP>((T *)a.dq + (((int64_t)b * a.Lq + c.i) * a.H + e * a.G + c.g) * a.D, a.D, dq, a.scale);
+    const float back = kNarrow<T> ? __builtin_amdgcn_exp2f(-power) : 1.0f;
+    if constexpr (SPLIT) store_column<float, DP>(a.part + ((split * (int64_t)a.B * a.E + be) * a.rows + c.row) * a.D, a.D, dq, back);
+    else store_column<T, DP>((T *)a.dq + (((int64_t)b * a.Lq + c.i) * a.H + e * a.G + c.g) * a.D, a.D, dq, a.scale * back);
   }
 }
 
@@ -701,6 +735,7 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv16(AttArgs a) {
   const T *qb = (const T *)a.q + b * a.qs[0] + (int64_t)e * a.G * a.qs[2], *gb = (const T *)a.go + b * a.gs[0] + (int64_t)e * a.G * a.gs[2];
   Stage<T, DP> staged;
   float lse = 0.0f, delta = 0.0f;
+  float times = power_of_2((int)kStart);   // what this column's dS and dk are multiplied by (kNarrow)
   const int n = !__syncthreads_or(on) ? 0 : WHOLE ? a.G * ((a.Lq + kTile - 1) / kTile) : (a.rows + kTile - 1) / kTile;   // (no kept key here: zeros)
   // as in walk_tiles: a tile of q beside the first half of the work, a tile of dO beside the second
   // the tile to load: with WHOLE from row i0 of head g0 (a head's last tile ends with it), else the rows from tile * kTile of the group's list
@@ -727,7 +762,7 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv16(AttArgs a) {
   };
   const auto store = [&](int which, int buffer) {
     staged.store(tiles[buffer] + which * kSize, ~0ull);
-    if (which == 0 && threadIdx.x < kTile) stats[buffer][0][threadIdx.x] = lse, stats[buffer][1][threadIdx.x] = -delta;
+    if (which == 0 && threadIdx.x < kTile) stats[buffer][0][threadIdx.x] = lse - kLiftP<T>, stats[buffer][1][threadIdx.x] = -delta;
   };
   if (n) {
     load(0, 0);
@@ -777,12 +812,27 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv16(AttArgs a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           p[4 * h + r] = (T)s[h][r];
-          ds[4 * h + r] = (T)(s[h][r] * dp[h][r]);
-          if constexpr (FINE) {
-            p_rest[4 * h + r] = (T)(s[h][r] - (float)p[4 * h + r]);
-            ds_rest[4 * h + r] = (T)(s[h][r] * dp[h][r] - (float)ds[4 * h + r]);
-          }
+          if constexpr (FINE) p_rest[4 * h + r] = (T)(s[h][r] - (float)p[4 * h + r]);
+          dp[h][r] *= s[h][r];
         }
+      }
+      if constexpr (kNarrow<T>) {
+        float most = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) most = fmaxf(most, fabsf(dp[r / 4][r % 4]));
+        if (__any(most * times > kMost)) {
+          most = fmaxf(most, __shfl_xor(most, 16)), most = fmaxf(most, __shfl_xor(most, 32));
+          const float now = most * times > kMost ? power_of_2(kAim - exponent_of(most)) : times;
+#pragma unroll
+          for (int d = 0; d < DP / 16; ++d) dk[d] *= now / times;
+          times = now;
+        }
+        dp[0] *= times, dp[1] *= times;
+      }
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        ds[r] = (T)dp[r / 4][r % 4];
+        if constexpr (FINE) ds_rest[r] = (T)(dp[r / 4][r % 4] - (float)ds[r]);
       }
 #pragma unroll
       for (int d = 0; d < DP / 16; ++d) {
@@ -805,11 +855,12 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv16(AttArgs a) {
   }
   if (!there) return;
   const int64_t to = (((int64_t)b * a.Lk + key) * a.E + e) * a.D;
+  const float dv_by = kNarrow<T> ? power_of_2(-(int)kLiftP<T>) : 1.0f, dk_by = kNarrow<T> ? a.scale * dv_by / times : a.scale;
 #pragma unroll
   for (int d = 0; d < DP / 16; ++d) {
     const int at = 16 * d + 4 * (lane >> 4);
-    const float x[4] = {dk[d][0] * a.scale, dk[d][1] * a.scale, dk[d][2] * a.scale, dk[d][3] * a.scale};
-    const float y[4] = {dv[d][0], dv[d][1], dv[d][2], dv[d][3]};
+    const float x[4] = {dk[d][0] * dk_by, dk[d][1] * dk_by, dk[d][2] * dk_by, dk[d][3] * dk_by};
+    const float y[4] = {dv[d][0] * dv_by, dv[d][1] * dv_by, dv[d][2] * dv_by, dv[d][3] * dv_by};
     store_n<4>((T *)a.dk + to + at, a.D - at, x);
     store_n<4>((T *)a.dv + to + at, a.D - at, y);
   }
@@ -848,6 +899,7 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv32(AttArgs a) {
   Stage<T, DP> staged;
   const Reader<DP> reader = Reader<DP>::wide(tiles);
   float lse = 0.0f, delta = 0.0f;
+  float times = power_of_2((int)kStart);   // what this column's dS and dk are multiplied by (kNarrow)
   const int n = !__syncthreads_or(on) ? 0 : WHOLE ? a.G * ((a.Lq + kTile - 1) / kTile) : (a.rows + kTile - 1) / kTile;   // (no kept key here: zeros)
   // as in walk_tiles: a tile of q beside the first half of the work, a tile of dO beside the second
   // the tile to load: with WHOLE from row i0 of head g0 (a head's last tile ends with it), else the rows from tile * kTile of the group's list
@@ -874,7 +926,7 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv32(AttArgs a) {
   };
   const auto store = [&](int which, int buffer) {
     staged.store(tiles[buffer] + which * kSize, ~0ull);
-    if (which == 0 && threadIdx.x < kTile) stats[buffer][0][threadIdx.x] = lse, stats[buffer][1][threadIdx.x] = -delta;
+    if (which == 0 && threadIdx.x < kTile) stats[buffer][0][threadIdx.x] = lse - kLiftP<T>, stats[buffer][1][threadIdx.x] = -delta;
   };
   if (n) {
     load(0, 0);
@@ -927,6 +979,19 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv32(AttArgs a) {
           if constexpr (FINE) dv[d] = mfma(c[half][d], rest_frag<T>(s, half), dv[d]);
         }
       dp *= s;
+      if constexpr (kNarrow<T>) {
+        float most = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(dp[r]));
+        if (__any(most * times > kMost)) {
+          most = fmaxf(most, other_half(most));
+          const float now = most * times > kMost ? power_of_2(kAim - exponent_of(most)) : times;
+#pragma unroll
+          for (int d = 0; d < DP / 32; ++d) dk[d] *= now / times;
+          times = now;
+        }
+        dp *= times;
+      }
       const V8 ds[2] = {to_frag<T>(dp, 0), to_frag<T>(dp, 1)};
       fence();
       if (t == 0) row_frags<T, DP>(r, 0, 1, qf);
@@ -947,8 +1012,9 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv32(AttArgs a) {
   }
   if (!there) return;
   const int64_t to = (((int64_t)b * a.Lk + key) * a.E + e) * a.D;
-  store_column<T, DP>((T *)a.dk + to, a.D, dk, a.scale);
-  store_column<T, DP>((T *)a.dv + to, a.D, dv, 1.0f);
+  const float dv_by = kNarrow<T> ? power_of_2(-(int)kLiftP<T>) : 1.0f, dk_by = kNarrow<T> ? a.scale * dv_by / times : a.scale;
+  store_column<T, DP>((T *)a.dk + to, a.D, dk, dk_by);
+  store_column<T, DP>((T *)a.dv + to, a.D, dv, dv_by);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------
