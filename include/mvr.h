@@ -497,6 +497,16 @@ int mvr_attend_tokens_forward(const mvr_attend_params *params, const void *q, co
 int mvr_attend_tokens_backward(const mvr_attend_params *params, const void *q, const void *k, const void *v,
                                const uint8_t *keep, const void *out, const float *lse, const void *grad_out, void *grad_q,
                                void *grad_k, void *grad_v, void *workspace, size_t workspace_bytes, mvr_stream_t stream);
+/* The same with what out's rounding left of it (out's type and shape), written by the forward and read by the backward: where a
+ * query's probabilities gather on few keys, grad_q and grad_k have half the error with it.  NULL: without, as above.  It goes
+ * with lse; up to 64 keys it is neither written nor read. */
+int mvr_attend_tokens_forward_rest(const mvr_attend_params *params, const void *q, const void *k, const void *v,
+                                   const uint8_t *keep, void *out, void *out_rest, float *lse, void *workspace,
+                                   size_t workspace_bytes, mvr_stream_t stream);
+int mvr_attend_tokens_backward_rest(const mvr_attend_params *params, const void *q, const void *k, const void *v,
+                                    const uint8_t *keep, const void *out, const void *out_rest, const float *lse,
+                                    const void *grad_out, void *grad_q, void *grad_k, void *grad_v, void *workspace,
+                                    size_t workspace_bytes, mvr_stream_t stream);
 
 #ifdef __cplusplus
 }

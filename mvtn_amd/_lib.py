@@ -87,6 +87,8 @@ PROTOTYPES = {
     "mvr_attend_tokens_workspace_bytes": (ctypes.c_size_t, [_AP, ctypes.c_int32]),
     "mvr_attend_tokens_forward": (ctypes.c_int, [_AP] + [_vp] * 7 + [ctypes.c_size_t, _vp]),
     "mvr_attend_tokens_backward": (ctypes.c_int, [_AP] + [_vp] * 11 + [ctypes.c_size_t, _vp]),
+    "mvr_attend_tokens_forward_rest": (ctypes.c_int, [_AP] + [_vp] * 8 + [ctypes.c_size_t, _vp]),
+    "mvr_attend_tokens_backward_rest": (ctypes.c_int, [_AP] + [_vp] * 12 + [ctypes.c_size_t, _vp]),
     "mvr_rotate_tokens_forward": (ctypes.c_int, [_RP] + [_vp] * 5),
     "mvr_rotate_tokens_backward": (ctypes.c_int, [_RP] + [_vp] * 7),
     "mvr_add_norm_tokens_forward": (ctypes.c_int, [_NP] + [_vp] * 11),
@@ -238,8 +240,8 @@ def token_op():
         lib = load()
         torch.ops.load_library(_build.build_torch_op(path=_build.TOKEN_OP_PATH))
         torch.ops.mvr_tokens.init([ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in
-                                   ("mvr_rotate_tokens_forward", "mvr_rotate_tokens_backward", "mvr_attend_tokens_workspace_bytes", "mvr_attend_tokens_forward",
-                                    "mvr_attend_tokens_backward", "mvr_add_norm_tokens_workspace_bytes", "mvr_add_norm_tokens_forward",
+                                   ("mvr_rotate_tokens_forward", "mvr_rotate_tokens_backward", "mvr_attend_tokens_workspace_bytes", "mvr_attend_tokens_forward_rest",
+                                    "mvr_attend_tokens_backward_rest", "mvr_add_norm_tokens_workspace_bytes", "mvr_add_norm_tokens_forward",
                                     "mvr_add_norm_tokens_backward", "mvr_last_error")])
         _TOKEN_OP = torch.ops.mvr_tokens
     return _TOKEN_OP

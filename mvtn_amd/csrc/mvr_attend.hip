@@ -47,6 +47,7 @@ struct AttArgs {
   const void *q, *k, *v, *o, *go;
   const uint8_t *keep;
   void *out, *dq, *dk, *dv;
+  void *rest;                    // what out's rounding left, in its type and layout; or null
   float *lse;                    // (B, heads, queries): log2 of the sum of exp2(scale log2(e) q k); +inf for a row without keys
   float *delta;                  // the same shape
   float *part, *part_lse;        // splits over the keys: (splits, B kv_heads rows, D) and (splits, B kv_heads rows)
@@ -398,6 +399,16 @@ __device__ __forceinline__ void store_column(U *p, int D, const f32x16 (&x)[DP /
       store_n<4>(p + at, D == DP ? 4 : D - at, v);
     }
 }
+// what store_column's rounding leaves of the same values
+template <typename T, int DP>
+__device__ __forceinline__ void store_column_rest(T *p, int D, const f32x16 (&x)[DP / 32], float f) {
+  f32x16 y[DP / 32];
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) y[d][r] = x[d][r] * f - (float)(T)(x[d][r] * f);
+  store_column<T, DP>(p, D, y, 1.0f);
+}
 // the scores of keys that are not there, replaced: a register's 32 + 32 lanes hold two keys, so their bits make its lane mask on the scalar unit
 __device__ __forceinline__ void mask_scores(f32x16 &s, unsigned long long m, int t, float by) {
   const unsigned bits = (unsigned)(m >> (32 * t));
@@ -414,15 +425,21 @@ __device__ __forceinline__ void mask_scores(f32x16 &s, unsigned long long m, int
 // (Following every new maximum, one of a wave's 64 columns has one in four tiles of five, at 68 multiplications each.)
 constexpr float kSlack = 8.0f;
 
+// LSE: the sum is also taken of the probabilities as they are, for lse: the backward's P would all be off by what rounding made of the sum, which
+// one large probability among them decides.  The output is divided by the sum of the rounded ones, which cancels that.  (Splits are weighted by lse.)
+// With `rest` the backward also has the output in more bits than its store: delta = rowsum(dO O) stands against dP, and where one probability is near 1
+// the difference is small.  Error of dQ over its store's alone, 1024 keys of 64, scores with a deviation of 1 / 3 / 6 / 10: 1.4 / 1.5 / 1.5 / 1.5 times, without
+// the two 1.4 / 1.9 / 2.5 / 3.1.  Forward and gradients with and without: 16 x 2352 tokens, 12 heads of 64, a quarter dropped, 1450 / 1407 us; 8 x 3920, 16
+// heads of 128, 5605 / 5520; 16 x 1000, 12 heads of 32 (the forward on two waves a SIMD in place of three) 210 / 196.
+//
 // FINE (here and in the backward), where all keys lie in one tile: P and dS enter their products, and P the sum, as two parts, a rounded value and what
 // its rounding left, and delta comes from P and dP in 32 bits.  Otherwise the gradients carry, beside the store's rounding, one of P and dS (1.4
-// times the store's error alone, at any length), and that of the sum and of the stored output in delta, which average out over many keys
-// but not over few (1.6 times with 12 keys and heads of 64; 1.0 with FINE).  It costs, forward / backward: 384 x 64 tokens, 12 heads of 64 on 4
+// times the store's error alone), and in dQ that of P in delta (to 1.5 where few keys have the sum; 1.0 with FINE).  It costs, forward / backward: 384 x 64 tokens, 12 heads of 64 on 4
 // 30.4 -> 31.6 / 76 -> 87 us; 16 heads of 128 107 -> 109 / 292 us both; 64 x 1000 queries over 48 keys 60.7 -> 65 / 164 -> 179 us.
 //
 // NS columns of 32 queries a wave: with two, every operand read from LDS serves two products, and one's exponentials run beside the other's
 // products
-template <typename T, int DP, int NS, bool SPLIT, bool WHOLE, bool FINE>
+template <typename T, int DP, int NS, bool SPLIT, bool WHOLE, bool FINE, bool LSE>
 __global__ __launch_bounds__(kBlock, 2) void k_attend(AttArgs a) {
   typedef typename Vec<T>::type V8;
   constexpr int kSize = Layout<DP>::kSize;
@@ -436,14 +453,14 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend(AttArgs a) {
   const int b = (int)(be / a.E), e = (int)(be - (int64_t)b * a.E);
   V8 q[NS][DP / 16];
   f32x16 o[NS][DP / 32];
-  float top[NS], sum[NS];   // of this lane's column; the sum over the rows this lane holds
+  float top[NS], sum[NS], sum_as_is[NS];   // of this lane's column; the sums over the rows this lane holds
 #pragma unroll
   for (int n = 0; n < NS; ++n) {
     const Column c = column_of(a, ct, n, 32 * NS);
     load_frags<T, DP>((const T *)a.q + b * a.qs[0] + c.i * a.qs[1] + (e * a.G + c.g) * a.qs[2], a, q[n]);
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) o[n][d] = 0.0f;
-    top[n] = -INFINITY, sum[n] = 0.0f;
+    top[n] = -INFINITY, sum[n] = sum_as_is[n] = 0.0f;
   }
   const T *kb = (const T *)a.k + b * a.ks[0] + e * a.ks[2], *vb = (const T *)a.v + b * a.vs[0] + e * a.vs[2];
   Stage<T, DP> staged;
@@ -462,6 +479,10 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend(AttArgs a) {
           const float off = top[n] == -INFINITY ? 0.0f : top[n] - kLift<T>;
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[n][t][r] = __builtin_amdgcn_exp2f(fmaf(s[n][t][r], a.c, -off));
+          if constexpr (LSE) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sum_as_is[n] += s[n][t][r];
+          }
           p[n][0] = to_frag<T>(s[n][t], 0), p[n][1] = to_frag<T>(s[n][t], 1);
           sum[n] = add_frag(p[n][1], add_frag(p[n][0], sum[n]));   // (of the probabilities as they enter the product)
 #pragma unroll
@@ -511,7 +532,7 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend(AttArgs a) {
 #pragma unroll
       for (int n = 0; n < NS; ++n) {
         const float f = __builtin_amdgcn_exp2f(top[n] - (now[n] == -INFINITY ? 0.0f : now[n]));
-        sum[n] *= f;
+        sum[n] *= f, sum_as_is[n] *= f;
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) o[n][d] *= f;
         top[n] = now[n];
@@ -523,16 +544,20 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend(AttArgs a) {
 #pragma unroll
   for (int n = 0; n < NS; ++n) {
     const Column c = column_of(a, ct, n, 32 * NS);
-    const float all = sum[n] + other_half(sum[n]);
+    const float all = sum[n] + other_half(sum[n]), as_is = LSE ? sum_as_is[n] + other_half(sum_as_is[n]) : all;
     if (!c.live) continue;
     const float inv = all > 0.0f ? 1.0f / all : all == 0.0f ? 0.0f : all;   // (a NaN stays one)
     if constexpr (SPLIT) {
       const int64_t line = (split * (int64_t)a.B * a.E + be) * a.rows + c.row;
       store_column<float, DP>(a.part + line * a.D, a.D, o[n], inv);
-      if (hi == 0) a.part_lse[line] = all == 0.0f ? -INFINITY : top[n] - kLift<T> + __builtin_amdgcn_logf(all);
+      if (hi == 0) a.part_lse[line] = all == 0.0f ? -INFINITY : top[n] - kLift<T> + __builtin_amdgcn_logf(as_is);
     } else {
-      store_column<T, DP>((T *)a.out + (((int64_t)b * a.Lq + c.i) * a.H + e * a.G + c.g) * a.D, a.D, o[n], inv);
-      if (a.lse && hi == 0) a.lse[be * a.rows + c.row] = all == 0.0f ? INFINITY : top[n] - kLift<T> + __builtin_amdgcn_logf(all);
+      const int64_t to = (((int64_t)b * a.Lq + c.i) * a.H + e * a.G + c.g) * a.D;
+      store_column<T, DP>((T *)a.out + to, a.D, o[n], inv);
+      if constexpr (LSE) {
+        if (a.rest) store_column_rest<T, DP>((T *)a.rest + to, a.D, o[n], inv);
+      }
+      if (a.lse && hi == 0) a.lse[be * a.rows + c.row] = all == 0.0f ? INFINITY : top[n] - kLift<T> + __builtin_amdgcn_logf(as_is);
     }
   }
 }
@@ -555,9 +580,13 @@ __global__ __launch_bounds__(kBlock) void k_attend_join(AttArgs a) {
   }
   const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
   const int64_t be = line / a.rows, row = line - be * a.rows, b = be / a.E, e = be - b * a.E, g = row / a.Lq, i = row - g * a.Lq;
-  T *p = (T *)a.out + ((b * a.Lq + i) * a.H + e * a.G + g) * a.D;
+  const int64_t to = ((b * a.Lq + i) * a.H + e * a.G + g) * a.D;
   for (int k = 0; k < 2; ++k)
-    if (lane + 64 * k < a.D) p[lane + 64 * k] = (T)(x[k] * inv);
+    if (lane + 64 * k < a.D) {
+      const T y = (T)(x[k] * inv);
+      ((T *)a.out)[to + lane + 64 * k] = y;
+      if (a.rest) ((T *)a.rest)[to + lane + 64 * k] = (T)(x[k] * inv - (float)y);
+    }
   if (a.lse && lane == 0) a.lse[line] = sum == 0.0f ? INFINITY : off + __builtin_amdgcn_logf(sum);
 }
 
@@ -587,12 +616,17 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dq(AttArgs a) {
   load_frags<T, DP>((const T *)a.q + b * a.qs[0] + c.i * a.qs[1] + h * a.qs[2], a, q);
   load_frags<T, DP>((const T *)a.go + b * a.gs[0] + c.i * a.gs[1] + h * a.gs[2], a, go);
   if constexpr (!FINE) {
-    V8 o[DP / 16];
-    load_frags<T, DP>((const T *)a.o + (((int64_t)b * a.Lq + c.i) * a.H + h) * a.D, a, o);
+    const int64_t at = (((int64_t)b * a.Lq + c.i) * a.H + h) * a.D;
+    const auto add = [&](const void *part) {
+      V8 o[DP / 16];
+      load_frags<T, DP>((const T *)part + at, a, o);
 #pragma unroll
-    for (int s = 0; s < DP / 16; ++s)
+      for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) delta += (float)o[s][k] * (float)go[s][k];
+        for (int k = 0; k < 8; ++k) delta += (float)o[s][k] * (float)go[s][k];
+    };
+    add(a.o);
+    if (a.rest) add(a.rest);
     delta += other_half(delta);
   }
   lse = c.live ? a.lse[be * a.rows + c.row] : INFINITY;
@@ -1066,28 +1100,25 @@ bool grid_of(AttArgs &a, int64_t columns, int per, int splits, unsigned &blocks)
   return n <= 0x7FFFFFFF;
 }
 
+template <typename T, int DP, bool SPLIT, bool FINE, bool LSE>
+void launch_attend(const AttArgs &a, unsigned n, hipStream_t st) {
+  const dim3 g(n), blk(kBlock);
+  constexpr int kWide = DP <= 64 ? 2 : 1;
+  if (a.wide) hipLaunchKernelGGL((k_attend<T, DP, kWide, SPLIT, true, FINE, LSE>), g, blk, 0, st, a);
+  else if (a.whole) hipLaunchKernelGGL((k_attend<T, DP, 1, SPLIT, true, FINE, LSE>), g, blk, 0, st, a);
+  else hipLaunchKernelGGL((k_attend<T, DP, 1, SPLIT, false, FINE, LSE>), g, blk, 0, st, a);
+}
+
 template <typename T, int DP>
 int launch_forward(AttArgs a, hipStream_t st) {
   unsigned n;
   if (!grid_of(a, a.rows, 32 * kWaves * (1 + a.wide), a.splits, n)) return bad("mvr_attend_tokens_forward: too many workgroups");
-  const dim3 g(n), blk(kBlock);
-  constexpr int kWide = DP <= 64 ? 2 : 1;
-  if (a.tiles == 1) {
-    if (a.wide) hipLaunchKernelGGL((k_attend<T, DP, kWide, false, true, true>), g, blk, 0, st, a);
-    else if (a.whole) hipLaunchKernelGGL((k_attend<T, DP, 1, false, true, true>), g, blk, 0, st, a);
-    else hipLaunchKernelGGL((k_attend<T, DP, 1, false, false, true>), g, blk, 0, st, a);
-    return launched("k_attend");
-  }
-  if (a.splits == 1) {
-    if (a.wide) hipLaunchKernelGGL((k_attend<T, DP, kWide, false, true, false>), g, blk, 0, st, a);
-    else if (a.whole) hipLaunchKernelGGL((k_attend<T, DP, 1, false, true, false>), g, blk, 0, st, a);
-    else hipLaunchKernelGGL((k_attend<T, DP, 1, false, false, false>), g, blk, 0, st, a);
-    return launched("k_attend");
-  }
-  if (a.wide) hipLaunchKernelGGL((k_attend<T, DP, kWide, true, true, false>), g, blk, 0, st, a);
-  else if (a.whole) hipLaunchKernelGGL((k_attend<T, DP, 1, true, true, false>), g, blk, 0, st, a);
-  else hipLaunchKernelGGL((k_attend<T, DP, 1, true, false, false>), g, blk, 0, st, a);
+  if (a.tiles == 1) launch_attend<T, DP, false, true, false>(a, n, st);   // (FINE's sum is the one of P as it is)
+  else if (a.splits > 1) launch_attend<T, DP, true, false, true>(a, n, st);
+  else if (a.lse) launch_attend<T, DP, false, false, true>(a, n, st);
+  else launch_attend<T, DP, false, false, false>(a, n, st);
   if (int rc = launched("k_attend")) return rc;
+  if (a.splits == 1) return MVR_OK;
   hipLaunchKernelGGL((k_attend_join<T>), dim3((unsigned)((lines(a) + kWaves - 1) / kWaves)), dim3(kBlock), 0, st, a);
   return launched("k_attend_join");
 }
@@ -1142,25 +1173,32 @@ extern "C" size_t mvr_attend_tokens_workspace_bytes(const mvr_attend_params *par
   return backward ? backward_bytes(a) : forward_bytes(a);
 }
 
-extern "C" int mvr_attend_tokens_forward(const mvr_attend_params *params, const void *q, const void *k, const void *v, const uint8_t *keep, void *out,
-                                         float *lse, void *workspace, size_t workspace_bytes, mvr_stream_t stream) {
+extern "C" int mvr_attend_tokens_forward_rest(const mvr_attend_params *params, const void *q, const void *k, const void *v, const uint8_t *keep, void *out,
+                                              void *out_rest, float *lse, void *workspace, size_t workspace_bytes, mvr_stream_t stream) {
   AttArgs a = {};
   if (int rc = att_args(a, params)) return rc;
   if (!q || !k || !v || !out) return bad("mvr_attend_tokens_forward: q, k, v and out must be given");
   if (out == q || out == k || out == v) return bad("mvr_attend_tokens_forward: out must not be an input");
+  if (out_rest && !lse) return bad("mvr_attend_tokens_forward: out_rest goes with lse");
+  if (out_rest && (out_rest == q || out_rest == k || out_rest == v || out_rest == out)) return bad("mvr_attend_tokens_forward: out_rest must be memory of its own");
   if ((keep != nullptr) != (params->keep_groups > 0)) return bad("mvr_attend_tokens_forward: keep goes with its groups");
   const size_t need = forward_bytes(a);
   if (need && (!workspace || workspace_bytes < need))
     return fail(MVR_ERR_WORKSPACE, "mvr_attend_tokens_forward: the workspace is smaller than mvr_attend_tokens_workspace_bytes says");
-  a.q = q, a.k = k, a.v = v, a.keep = keep, a.out = out, a.lse = lse;
+  a.q = q, a.k = k, a.v = v, a.keep = keep, a.out = out, a.rest = out_rest, a.lse = lse;
   a.part = (float *)workspace, a.part_lse = (float *)((char *)workspace + align256(lines(a) * a.splits * a.D * 4));
   const hipStream_t st = (hipStream_t)stream;
   return params->type == MVR_TYPE_HALF ? MVR_ATT_DIMS(launch_forward, f16, a, st) : MVR_ATT_DIMS(launch_forward, bf16, a, st);
 }
 
-extern "C" int mvr_attend_tokens_backward(const mvr_attend_params *params, const void *q, const void *k, const void *v, const uint8_t *keep,
-                                          const void *out, const float *lse, const void *grad_out, void *grad_q, void *grad_k, void *grad_v,
-                                          void *workspace, size_t workspace_bytes, mvr_stream_t stream) {
+extern "C" int mvr_attend_tokens_forward(const mvr_attend_params *params, const void *q, const void *k, const void *v, const uint8_t *keep, void *out,
+                                         float *lse, void *workspace, size_t workspace_bytes, mvr_stream_t stream) {
+  return mvr_attend_tokens_forward_rest(params, q, k, v, keep, out, nullptr, lse, workspace, workspace_bytes, stream);
+}
+
+extern "C" int mvr_attend_tokens_backward_rest(const mvr_attend_params *params, const void *q, const void *k, const void *v, const uint8_t *keep,
+                                               const void *out, const void *out_rest, const float *lse, const void *grad_out, void *grad_q,
+                                               void *grad_k, void *grad_v, void *workspace, size_t workspace_bytes, mvr_stream_t stream) {
   AttArgs a = {};
   if (int rc = att_args(a, params)) return rc;
   if (!q || !k || !v || !out || !lse || !grad_out || !grad_q || !grad_k || !grad_v)
@@ -1168,8 +1206,14 @@ extern "C" int mvr_attend_tokens_backward(const mvr_attend_params *params, const
   if ((keep != nullptr) != (params->keep_groups > 0)) return bad("mvr_attend_tokens_backward: keep goes with its groups");
   if (!workspace || workspace_bytes < backward_bytes(a))
     return fail(MVR_ERR_WORKSPACE, "mvr_attend_tokens_backward: the workspace is smaller than mvr_attend_tokens_workspace_bytes says");
-  a.q = q, a.k = k, a.v = v, a.keep = keep, a.o = out, a.lse = const_cast<float *>(lse), a.go = grad_out, a.dq = grad_q, a.dk = grad_k, a.dv = grad_v;
+  a.q = q, a.k = k, a.v = v, a.keep = keep, a.o = out, a.rest = const_cast<void *>(out_rest), a.lse = const_cast<float *>(lse), a.go = grad_out, a.dq = grad_q, a.dk = grad_k, a.dv = grad_v;
   a.delta = (float *)workspace, a.part = (float *)((char *)workspace + align256(lines(a) * 4));
   const hipStream_t st = (hipStream_t)stream;
   return params->type == MVR_TYPE_HALF ? MVR_ATT_DIMS(launch_backward, f16, a, st) : MVR_ATT_DIMS(launch_backward, bf16, a, st);
+}
+
+extern "C" int mvr_attend_tokens_backward(const mvr_attend_params *params, const void *q, const void *k, const void *v, const uint8_t *keep,
+                                          const void *out, const float *lse, const void *grad_out, void *grad_q, void *grad_k, void *grad_v,
+                                          void *workspace, size_t workspace_bytes, mvr_stream_t stream) {
+  return mvr_attend_tokens_backward_rest(params, q, k, v, keep, out, nullptr, lse, grad_out, grad_q, grad_k, grad_v, workspace, workspace_bytes, stream);
 }

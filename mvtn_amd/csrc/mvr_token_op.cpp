@@ -28,8 +28,8 @@ struct Entry {
   decltype(&mvr_rotate_tokens_forward) rotate = nullptr;
   decltype(&mvr_rotate_tokens_backward) rotate_backward = nullptr;
   decltype(&mvr_attend_tokens_workspace_bytes) attend_bytes = nullptr;
-  decltype(&mvr_attend_tokens_forward) attend = nullptr;
-  decltype(&mvr_attend_tokens_backward) attend_backward = nullptr;
+  decltype(&mvr_attend_tokens_forward_rest) attend = nullptr;
+  decltype(&mvr_attend_tokens_backward_rest) attend_backward = nullptr;
   decltype(&mvr_add_norm_tokens_workspace_bytes) norm_bytes = nullptr;
   decltype(&mvr_add_norm_tokens_forward) norm = nullptr;
   decltype(&mvr_add_norm_tokens_backward) norm_backward = nullptr;
@@ -182,15 +182,15 @@ mvr_attend_params attend_params(const Tensor &q, const Tensor &k, const Tensor &
 
 Tensor workspace(size_t bytes, const Tensor &like) { return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor(); }
 
-// q, k, v with packed rows; lse: undefined where no backward follows
-Tensor attend_forward(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &keep, double scale, const Tensor &lse, int64_t stream) {
+// q, k, v with packed rows; rest, lse: undefined where no backward follows
+Tensor attend_forward(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &keep, double scale, const Tensor &rest, const Tensor &lse, int64_t stream) {
   Tensor out = at::empty(q.sizes(), q.options());
   if (k.size(1) == 0) return out.zero_();
   if (out.numel() == 0) return out;
   const mvr_attend_params p = attend_params(q, k, v, keep, Tensor(), scale);
   const size_t bytes = g_entry.attend_bytes(&p, 0);
   const Tensor ws = workspace(bytes, q);
-  check(g_entry.attend(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), (const uint8_t *)ptr(keep), out.data_ptr(), fptr(lse), ptr(ws), bytes, stream_of(stream)),
+  check(g_entry.attend(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), (const uint8_t *)ptr(keep), out.data_ptr(), ptr(rest), fptr(lse), ptr(ws), bytes, stream_of(stream)),
         "mvr_attend_tokens_forward");
   return out;
 }
@@ -201,15 +201,16 @@ struct Attend : public torch::autograd::Function<Attend> {
     const c10::DeviceGuard guard(q_.device());
     const Tensor q = rows_packed(q_), k = rows_packed(k_), v = rows_packed(v_);
     const Tensor lse = at::empty({q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
-    Tensor out = attend_forward(q, k, v, keep, scale, lse, stream);
-    ctx->save_for_backward({q, k, v, keep, out, lse});
+    const Tensor rest = k.size(1) > 64 ? at::empty(q.sizes(), q.options()) : Tensor();   // (over so few keys the backward does without)
+    Tensor out = attend_forward(q, k, v, keep, scale, rest, lse, stream);
+    ctx->save_for_backward({q, k, v, keep, out, lse, rest});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["stream"] = stream;
     return out;
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     const auto s = ctx->get_saved_variables();
-    const Tensor &q = s[0], &k = s[1], &v = s[2], &keep = s[3], &out = s[4], &lse = s[5];
+    const Tensor &q = s[0], &k = s[1], &v = s[2], &keep = s[3], &out = s[4], &lse = s[5], &rest = s[6];
     const c10::DeviceGuard guard(q.device());
     Tensor gq = at::empty(q.sizes(), q.options()), gk = at::empty(k.sizes(), k.options()), gv = at::empty(v.sizes(), v.options());
     if (out.numel() && k.size(1)) {
@@ -217,7 +218,7 @@ struct Attend : public torch::autograd::Function<Attend> {
       const mvr_attend_params p = attend_params(q, k, v, keep, grad, ctx->saved_data["scale"].toDouble());
       const size_t bytes = g_entry.attend_bytes(&p, 1);
       const Tensor ws = workspace(bytes, q);
-      check(g_entry.attend_backward(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), (const uint8_t *)ptr(keep), out.data_ptr(), lse.data_ptr<float>(),
+      check(g_entry.attend_backward(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), (const uint8_t *)ptr(keep), out.data_ptr(), ptr(rest), lse.data_ptr<float>(),
                                     grad.data_ptr(), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), ptr(ws), bytes, stream_of(ctx->saved_data["stream"].toInt())),
             "mvr_attend_tokens_backward");
     } else {
@@ -246,7 +247,7 @@ Tensor attend_tokens(const Tensor &q, const Tensor &k, const Tensor &v, const Ma
   if (keep.defined()) keep = (keep.scalar_type() == at::kBool || keep.scalar_type() == at::kByte ? keep : keep.ne(0)).contiguous();
   if (wants_grad({&q, &k, &v})) return Attend::apply(q, k, v, some(keep), scale, stream);
   const c10::DeviceGuard guard(q.device());
-  return attend_forward(rows_packed(q), rows_packed(k), rows_packed(v), keep, scale, Tensor(), stream);
+  return attend_forward(rows_packed(q), rows_packed(k), rows_packed(v), keep, scale, Tensor(), Tensor(), stream);
 }
 
 // ---- norms around a block ----------------------------------------------------------------------------------------------

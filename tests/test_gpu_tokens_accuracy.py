@@ -65,6 +65,20 @@ def _check(got, want, var, dtype):
         assert far <= room + 2.0 ** -16 * w.norm(), (name, float(far / store), float(room / store))   # (32-bit scores, exponentials and sums: some 2^-18)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("spread", [1.0, 3.0, 6.0, 10.0])
+@pytest.mark.parametrize("B,Lq,Lk,H,E,D,groups", [(1, 512, 1024, 2, 1, 64, 0), (1, 300, 2352, 1, 1, 128, 12), (2, 200, 500, 2, 2, 41, 0), (4, 3, 3000, 8, 2, 64, 20), (4, 2, 3000, 4, 4, 100, 0), (2, 300, 100, 2, 1, 32, 0)])
+def test_gradients_of_peaked_probabilities(dtype, spread, B, Lq, Lk, H, E, D, groups):
+    """Scores with a deviation of 1 to 10: a few keys take nearly all.  Then dP - delta is a small difference, and neither the output's store nor the rounding
+    of the sum may enter it."""
+    g = _gen(74)
+    q, k, v, do = (_randn(g, *s, dtype=dtype) for s in ((B, Lq, H, D), (B, Lk, E, D), (B, Lk, E, D), (B, Lq, H, D)))
+    keep = torch.rand(B, groups, generator=g, device=_dev()) < 0.7 if groups else None
+    scale = spread * D ** -0.5
+    want, var = _sizes(q, k, v, do, scale, keep)
+    _check(_call(q, k, v, do, keep, scale), want, var, dtype)
+
+
 @pytest.mark.parametrize("size", [1.0, 1e-2, 1e-3, 1e-4])
 @pytest.mark.parametrize("B,Lq,Lk,H,E,D", [(1, 300, 2352, 2, 1, 64), (2, 200, 1500, 1, 1, 128), (4, 1, 3920, 8, 4, 128), (1, 64, 30000, 1, 1, 32), (2, 500, 60, 2, 2, 64), (1, 700, 50, 4, 1, 104)])
 def test_float16_gradients_of_any_size(size, B, Lq, Lk, H, E, D):
