@@ -888,6 +888,10 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv16(AttArgs a) {
     lds_barrier();
   }
   if (!there) return;
+  if (!on) {   // (P = 0 times what dO or q hold is not 0 where they hold infinities)
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) dk[d] = dv[d] = 0.0f;
+  }
   const int64_t to = (((int64_t)b * a.Lk + key) * a.E + e) * a.D;
   const float dv_by = kNarrow<T> ? power_of_2(-(int)kLiftP<T>) : 1.0f, dk_by = kNarrow<T> ? a.scale * dv_by / times : a.scale;
 #pragma unroll
@@ -1045,6 +1049,10 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv32(AttArgs a) {
     lds_barrier();
   }
   if (!there) return;
+  if (!on) {   // (as above)
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) dk[d] = dv[d] = 0.0f;
+  }
   const int64_t to = (((int64_t)b * a.Lk + key) * a.E + e) * a.D;
   const float dv_by = kNarrow<T> ? power_of_2(-(int)kLiftP<T>) : 1.0f, dk_by = kNarrow<T> ? a.scale * dv_by / times : a.scale;
   store_column<T, DP>((T *)a.dk + to, a.D, dk, dk_by);
