@@ -88,9 +88,9 @@ void strides(int64_t (&to)[3], const Tensor &t) {
 }
 mvr_stream_t stream_of(int64_t s) { return reinterpret_cast<mvr_stream_t>(s); }
 
-// A gradient that somebody asks to differentiate again fails there, and not silently
-variable_list once(variable_list out, const variable_list &grads) {
-  bool again = false;
+// A gradient that somebody asks to differentiate again fails there, and not silently.  again: it depends on inputs that require grad, not on the
+// incoming gradients alone
+variable_list once(variable_list out, const variable_list &grads, bool again) {
   for (const Tensor &g : grads) again = again || (g.defined() && g.requires_grad());
   if (!at::GradMode::is_enabled() || !again) return out;
   variable_list in;
@@ -149,7 +149,7 @@ struct Rotate : public torch::autograd::Function<Rotate> {
     } else if (gp.defined()) {
       gp.zero_();
     }
-    return once({gx, gp, Tensor(), Tensor(), Tensor(), Tensor()}, grads);
+    return once({gx, gp, Tensor(), Tensor(), Tensor(), Tensor()}, grads, x.defined());   // (without the positions' a gradient is linear in dy)
   }
 };
 
@@ -224,7 +224,7 @@ struct Attend : public torch::autograd::Function<Attend> {
     } else {
       gq.zero_(), gk.zero_(), gv.zero_();
     }
-    return once({gq, gk, gv, Tensor(), Tensor(), Tensor()}, grads);
+    return once({gq, gk, gv, Tensor(), Tensor(), Tensor()}, grads, q.requires_grad() || k.requires_grad());   // (v's alone is linear in dO)
   }
 };
 
@@ -282,7 +282,9 @@ struct AddNorm : public torch::autograd::Function<AddNorm> {
     ctx->saved_data["params"] = params;
     ctx->saved_data["stream"] = stream;
     ctx->saved_data["need"] = std::vector<int64_t>{weight.requires_grad(), bias.defined() && bias.requires_grad(), post.defined() && post.requires_grad(),
-                                                   gate.defined() && gate.requires_grad()};
+                                                   gate.defined() && gate.requires_grad(),
+                                                   // (weight's and bias' alone are linear in dz)
+                                                   residual.requires_grad() || branch.requires_grad() || (post.defined() && post.requires_grad()) || (gate.defined() && gate.requires_grad())};
     return {y, z};
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
@@ -309,7 +311,7 @@ struct AddNorm : public torch::autograd::Function<AddNorm> {
       for (const Tensor *t : {&gw, &gbias, &gpost, &ggate})
         if (t->defined()) t->zero_();
     }
-    return once({gr, gb, gw, gbias, gpost, ggate, Tensor(), Tensor(), Tensor()}, grads);
+    return once({gr, gb, gw, gbias, gpost, ggate, Tensor(), Tensor(), Tensor()}, grads, need[4]);
   }
 };
 

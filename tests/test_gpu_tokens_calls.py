@@ -35,3 +35,24 @@ def test_dropped_keys_get_zero_beside_infinite_rows(dtype, Lq, Lk, H, E, D, grou
     got = _attention(q, k, v, do, keep)
     assert not torch.isfinite(got[2][0][~gone[0]][:, 0]).all() and not torch.isfinite(got[3][0][~gone[0]][:, 0]).all()
     assert not got[2][gone].any() and not got[3][gone].any()   # (any() of a NaN is true)
+
+
+def test_a_penalty_on_gradients_is_noticed():
+    """A gradient with create_graph and a constant gradient above it depends on the inputs all the same: its use in a loss fails, it is not a constant."""
+    g = _gen(91)
+    x, pos = _randn(g, 1, 4, 2, 8).requires_grad_(), _randn(g, 4, 1).requires_grad_()
+    h, w = _randn(g, 1, 4, 2, 8, dtype=torch.bfloat16).requires_grad_(), _randn(g, 8).requires_grad_()
+    v = _randn(g, 1, 4, 2, 8, dtype=torch.bfloat16).requires_grad_()
+    rotary = tokens.TokenRotary((4,))
+    for out, leaf in ((rotary(x, pos), x), (rotary(x, pos), pos), (tokens.attend_tokens(h, h, h), h), (tokens.attend_tokens(h.detach(), h, h.detach()), h),
+                      (tokens.add_norm_tokens(x, x, w)[1], x), (tokens.add_norm_tokens(x.detach(), x.detach(), w.detach(), gate=w)[0], w)):
+        first, = torch.autograd.grad(out.float().sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiated"):
+            (out.float().sum() + first.float().square().sum()).backward()
+    # gradients that do not depend on what requires grad are constants, and may be used as such
+    for out, leaf in ((rotary(x, pos.detach()), x), (tokens.attend_tokens(h.detach(), h.detach(), v), v), (tokens.add_norm_tokens(x.detach(), x.detach(), w)[1], w)):
+        first, = torch.autograd.grad(out.float().sum(), leaf, create_graph=True)
+        assert not first.requires_grad
+        leaf.grad = None
+        (out.float().sum() + first.float().square().sum()).backward()
+        assert torch.equal(leaf.grad, first)
