@@ -78,6 +78,12 @@ bool wants_grad(std::initializer_list<const Tensor *> ts) {
     if (t->defined() && t->requires_grad()) return true;
   return false;
 }
+// tangents would be dropped, the result's derivative taken for 0
+void no_forward_mode(std::initializer_list<const Tensor *> ts) {
+  for (const Tensor *t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(/*level=*/0).defined(),
+                                "mvtn_amd.tokens: these operators have no forward-mode derivative (the reverse mode has all of them)");
+}
 bool in_32_bits(const Tensor &t) {   // the C ABI's sizes
   for (int64_t n : t.sizes())
     if (n > 0x7FFFFFFF) return false;
@@ -162,6 +168,7 @@ Tensor rotate_tokens(const Tensor &x, const Tensor &positions_, const Tensor &tu
   const int64_t dims = positions_.dim();
   TORCH_CHECK_VALUE((dims == 2 || dims == 3) && positions_.size(-2) == L && positions_.size(-1) == axes && (dims == 2 || positions_.size(0) == 1 || positions_.size(0) == B),
                     "positions are (B, L, axes), (1, L, axes) or (L, axes) with L = ", L, " and ", axes, " axes");
+  no_forward_mode({&x, &positions_});
   same_device(x, {&positions_});
   const Tensor positions = positions_.to(at::kFloat).expand({B, L, axes});
   if (wants_grad({&x, &positions})) return Rotate::apply(x, positions, turns, sections, interleaved, stream);
@@ -243,6 +250,7 @@ Tensor attend_tokens(const Tensor &q, const Tensor &k, const Tensor &v, const Ma
     TORCH_CHECK_VALUE(keep.dim() == 2 && keep.size(0) == B && keep.size(1) >= 1 && Lk % keep.size(1) == 0, "keep is (B, G) with G a divisor of the ", Lk, " keys");
     TORCH_CHECK_VALUE(!keep.requires_grad(), "keep is a mask: it gets no gradient");
   }
+  no_forward_mode({&q, &k, &v});
   same_device(q, {&k, &v, &keep});
   if (keep.defined()) keep = (keep.scalar_type() == at::kBool || keep.scalar_type() == at::kByte ? keep : keep.ne(0)).contiguous();
   if (wants_grad({&q, &k, &v})) return Attend::apply(q, k, v, some(keep), scale, stream);
@@ -345,6 +353,7 @@ std::vector<Tensor> add_norm_tokens(const Tensor &residual, const Tensor &branch
     TORCH_CHECK_VALUE(!draws.requires_grad(), "scale holds draws: it gets no gradient (put what is learned into gate)");
     TORCH_CHECK_VALUE(draws.numel() >= 1 && rows % draws.numel() == 0, "scale has ", draws.numel(), " draws, which do not divide the ", rows, " rows");
   }
+  no_forward_mode({&residual, &branch, &weight, &bias, &post, &gate});
   same_device(residual, {&branch, &weight, &bias, &post, &gate, &draws});
   if (draws.defined()) draws = draws.to(at::kFloat).contiguous();
   mvr_norm_params p;

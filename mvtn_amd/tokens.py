@@ -9,7 +9,7 @@ with their backward passes (`mvr_rotate_tokens_*`, `mvr_attend_tokens_*`, `mvr_a
 
 Tokens are ordered view by view: l = (v * rows + row) * cols + col.  All tensors of a call live on one GPU; the work goes to that GPU's current
 stream, memory comes from torch's allocator, nothing synchronises.  Arguments that do not fit raise ValueError, tensors that are not on the GPU
-RuntimeError.  Gradients repeat bit by bit; they cannot be differentiated again.
+RuntimeError.  Gradients repeat bit by bit; they cannot be differentiated again, and there is no forward mode: both raise.
 
 A step may be captured into a HIP graph, backward included, if its leaves are made (detached) inside the capture or no eager graph of the same leaves
 is alive: torch would otherwise hand the capture's gradients to that graph's stream."""

@@ -1,5 +1,35 @@
 """CPU (-m "not gpu"): further calls of the operators on view tokens that are refused, or answered, before anything reaches the GPU."""
-from mvtn_amd import _lib
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+from mvtn_amd import _lib, tokens
+
+
+def _calls(dtype=torch.float32):
+    """(call, inputs that are differentiated) of each operator, on the CPU."""
+    r = lambda *s: torch.randn(*s, dtype=dtype)  # noqa: E731
+    rotary, h = tokens.TokenRotary((2, 1)), lambda *s: torch.randn(*s).half()  # noqa: E731
+    return [(rotary, [r(2, 3, 1, 8), r(3, 2)]), (tokens.attend_tokens, [h(2, 3, 2, 8), h(2, 6, 2, 8), h(2, 6, 2, 8)]),
+            (lambda a, b, w, bias, post, gate: tokens.add_norm_tokens(a, b, w, bias, post, gate, kind="layer"),
+             [r(2, 6, 8), r(2, 6, 8), r(8), r(8), r(8), r(2, 8)])]
+
+
+@pytest.mark.parametrize("which", range(3))
+def test_forward_mode_is_refused(which):
+    """Tangents are not carried on, so they may not be dropped: with any input, whether it requires grad or not, under no_grad too."""
+    call, inputs = _calls()[which]
+    for k in range(len(inputs)):
+        for needs in (False, True):
+            with forward_ad.dual_level():
+                args = list(inputs)
+                args[k] = forward_ad.make_dual(inputs[k].clone().requires_grad_(needs), torch.ones_like(inputs[k]))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(*args)
+                with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(*args)
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(call, tuple(inputs), tuple(torch.ones_like(t) for t in inputs))
 
 
 def test_attention_c_abi_with_the_rest_refuses_before_any_launch():
