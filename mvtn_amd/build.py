@@ -191,9 +191,11 @@ def build_torch_op(force=False, path=TORCH_OP_PATH):
             if not force and torch_op_is_current(path):
                 return path
             tmp = "%s.tmp.%d" % (path, os.getpid())
+            # (torch's stream header includes HIP's; the mesh step is handed its stream)
+            hip = ["-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-I" + os.path.join(ce.ROCM_HOME or "/opt/rocm", "include")] if path == TOKEN_OP_PATH else []
             cmd = (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)] +
-                   ["-I" + d for d in ce.include_paths()] + [_torch_op_sources(path)[0], "-o", tmp] +
-                   ["-L" + d for d in ce.library_paths()] + ["-ltorch", "-ltorch_cpu", "-lc10"])
+                   ["-I" + d for d in ce.include_paths()] + hip + [_torch_op_sources(path)[0], "-o", tmp] +
+                   ["-L" + d for d in ce.library_paths()] + ["-ltorch", "-ltorch_cpu", "-lc10"] + (["-lc10_hip"] if hip else []))
             try:
                 r = subprocess.run(cmd, capture_output=True, text=True)
                 if r.returncode != 0:

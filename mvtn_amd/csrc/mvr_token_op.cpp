@@ -3,10 +3,11 @@
 // autograd functions over ctypes, a forward and backward cost 110-160 us of host time, against 35-130 us on the GPU).
 //
 // Argument checks, allocation and the calls of the C ABI (include/mvr.h); no arithmetic.  The entry points' addresses are handed over
-// by mvtn_amd/_lib.py: this file does not link against libmvr_hip.so, and that library stays free of torch types.  What Python sees: ValueError
+// by mvtn_amd/_lib.py: this file does not link against libmvr_hip.so, and that library stays free of torch types.  (libc10_hip: torch's current stream.)  What Python sees: ValueError
 // for arguments that do not fit, RuntimeError for tensors that are not on the GPU and for errors of the library.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
@@ -92,7 +93,8 @@ bool in_32_bits(const Tensor &t) {   // the C ABI's sizes
 void strides(int64_t (&to)[3], const Tensor &t) {
   for (int k = 0; k < 3; ++k) to[k] = t.stride(k);
 }
-mvr_stream_t stream_of(int64_t s) { return reinterpret_cast<mvr_stream_t>(s); }
+// the stream that is current on the tensor's GPU when the work is issued (in a backward: the forward's, as the engine makes it current)
+mvr_stream_t stream_of(const Tensor &t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
 // A gradient that somebody asks to differentiate again fails there, and not silently.  again: it depends on inputs that require grad, not on the
 // incoming gradients alone
@@ -119,24 +121,22 @@ mvr_rotary_params rotary_params(const Tensor &x, const Tensor &grad, const Tenso
   return p;
 }
 
-Tensor rotate_forward(const Tensor &x_, const Tensor &positions_, const Tensor &turns, at::IntArrayRef sections, bool interleaved, int64_t stream) {
+Tensor rotate_forward(const Tensor &x_, const Tensor &positions_, const Tensor &turns, at::IntArrayRef sections, bool interleaved) {
   const c10::DeviceGuard guard(x_.device());
   Tensor out = at::empty(x_.sizes(), x_.options());
   if (out.numel() == 0) return out;
   const Tensor x = rows_packed(x_), positions = rows_packed(positions_);
   const mvr_rotary_params p = rotary_params(x, Tensor(), positions, sections, interleaved);
-  check(g_entry.rotate(&p, turns.data_ptr<double>(), x.data_ptr(), positions.data_ptr<float>(), out.data_ptr(), stream_of(stream)), "mvr_rotate_tokens_forward");
+  check(g_entry.rotate(&p, turns.data_ptr<double>(), x.data_ptr(), positions.data_ptr<float>(), out.data_ptr(), stream_of(x)), "mvr_rotate_tokens_forward");
   return out;
 }
 
 struct Rotate : public torch::autograd::Function<Rotate> {
-  static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &positions, const Tensor &turns, std::vector<int64_t> sections, bool interleaved,
-                        int64_t stream) {
-    Tensor out = rotate_forward(x, positions, turns, sections, interleaved, stream);
+  static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &positions, const Tensor &turns, std::vector<int64_t> sections, bool interleaved) {
+    Tensor out = rotate_forward(x, positions, turns, sections, interleaved);
     ctx->save_for_backward({positions.requires_grad() ? x : Tensor(), positions, turns});
     ctx->saved_data["sections"] = sections;
     ctx->saved_data["interleaved"] = interleaved;
-    ctx->saved_data["stream"] = stream;
     return out;
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
@@ -149,17 +149,16 @@ struct Rotate : public torch::autograd::Function<Rotate> {
     if (gx.numel()) {
       const auto sections = ctx->saved_data["sections"].toIntVector();
       const mvr_rotary_params p = rotary_params(x.defined() ? x : grad, grad, positions, sections, ctx->saved_data["interleaved"].toBool());
-      check(g_entry.rotate_backward(&p, turns.data_ptr<double>(), ptr(x), positions.data_ptr<float>(), grad.data_ptr(), gx.data_ptr(), fptr(gp),
-                                    stream_of(ctx->saved_data["stream"].toInt())),
+      check(g_entry.rotate_backward(&p, turns.data_ptr<double>(), ptr(x), positions.data_ptr<float>(), grad.data_ptr(), gx.data_ptr(), fptr(gp), stream_of(grad)),
             "mvr_rotate_tokens_backward");
     } else if (gp.defined()) {
       gp.zero_();
     }
-    return once({gx, gp, Tensor(), Tensor(), Tensor(), Tensor()}, grads, x.defined());   // (without the positions' a gradient is linear in dy)
+    return once({gx, gp, Tensor(), Tensor(), Tensor()}, grads, x.defined());   // (without the positions' a gradient is linear in dy)
   }
 };
 
-Tensor rotate_tokens(const Tensor &x, const Tensor &positions_, const Tensor &turns, std::vector<int64_t> sections, bool interleaved, int64_t stream) {
+Tensor rotate_tokens(const Tensor &x, const Tensor &positions_, const Tensor &turns, std::vector<int64_t> sections, bool interleaved) {
   TORCH_CHECK_VALUE(x.dim() == 4, "x is (B, L, H, D)");
   const int64_t B = x.size(0), L = x.size(1), D = x.size(3), pairs = turns.numel(), axes = (int64_t)sections.size();
   TORCH_CHECK_VALUE(type_of(x) >= 0, "x must be float32, float16 or bfloat16, not ", x.scalar_type());
@@ -171,8 +170,8 @@ Tensor rotate_tokens(const Tensor &x, const Tensor &positions_, const Tensor &tu
   no_forward_mode({&x, &positions_});
   same_device(x, {&positions_});
   const Tensor positions = positions_.to(at::kFloat).expand({B, L, axes});
-  if (wants_grad({&x, &positions})) return Rotate::apply(x, positions, turns, sections, interleaved, stream);
-  return rotate_forward(x, positions, turns, sections, interleaved, stream);
+  if (wants_grad({&x, &positions})) return Rotate::apply(x, positions, turns, sections, interleaved);
+  return rotate_forward(x, positions, turns, sections, interleaved);
 }
 
 // ---- attention ---------------------------------------------------------------------------------------------------------
@@ -190,29 +189,28 @@ mvr_attend_params attend_params(const Tensor &q, const Tensor &k, const Tensor &
 Tensor workspace(size_t bytes, const Tensor &like) { return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor(); }
 
 // q, k, v with packed rows; rest, lse: undefined where no backward follows
-Tensor attend_forward(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &keep, double scale, const Tensor &rest, const Tensor &lse, int64_t stream) {
+Tensor attend_forward(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &keep, double scale, const Tensor &rest, const Tensor &lse) {
   Tensor out = at::empty(q.sizes(), q.options());
   if (k.size(1) == 0) return out.zero_();
   if (out.numel() == 0) return out;
   const mvr_attend_params p = attend_params(q, k, v, keep, Tensor(), scale);
   const size_t bytes = g_entry.attend_bytes(&p, 0);
   const Tensor ws = workspace(bytes, q);
-  check(g_entry.attend(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), (const uint8_t *)ptr(keep), out.data_ptr(), ptr(rest), fptr(lse), ptr(ws), bytes, stream_of(stream)),
+  check(g_entry.attend(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), (const uint8_t *)ptr(keep), out.data_ptr(), ptr(rest), fptr(lse), ptr(ws), bytes, stream_of(q)),
         "mvr_attend_tokens_forward");
   return out;
 }
 
 struct Attend : public torch::autograd::Function<Attend> {
-  static Tensor forward(AutogradContext *ctx, const Tensor &q_, const Tensor &k_, const Tensor &v_, const MaybeTensor &keep_, double scale, int64_t stream) {
+  static Tensor forward(AutogradContext *ctx, const Tensor &q_, const Tensor &k_, const Tensor &v_, const MaybeTensor &keep_, double scale) {
     const Tensor keep = or_none(keep_);
     const c10::DeviceGuard guard(q_.device());
     const Tensor q = rows_packed(q_), k = rows_packed(k_), v = rows_packed(v_);
     const Tensor lse = at::empty({q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
     const Tensor rest = k.size(1) > 64 ? at::empty(q.sizes(), q.options()) : Tensor();   // (over so few keys the backward does without)
-    Tensor out = attend_forward(q, k, v, keep, scale, rest, lse, stream);
+    Tensor out = attend_forward(q, k, v, keep, scale, rest, lse);
     ctx->save_for_backward({q, k, v, keep, out, lse, rest});
     ctx->saved_data["scale"] = scale;
-    ctx->saved_data["stream"] = stream;
     return out;
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
@@ -226,16 +224,16 @@ struct Attend : public torch::autograd::Function<Attend> {
       const size_t bytes = g_entry.attend_bytes(&p, 1);
       const Tensor ws = workspace(bytes, q);
       check(g_entry.attend_backward(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), (const uint8_t *)ptr(keep), out.data_ptr(), ptr(rest), lse.data_ptr<float>(),
-                                    grad.data_ptr(), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), ptr(ws), bytes, stream_of(ctx->saved_data["stream"].toInt())),
+                                    grad.data_ptr(), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), ptr(ws), bytes, stream_of(q)),
             "mvr_attend_tokens_backward");
     } else {
       gq.zero_(), gk.zero_(), gv.zero_();
     }
-    return once({gq, gk, gv, Tensor(), Tensor(), Tensor()}, grads, q.requires_grad() || k.requires_grad());   // (v's alone is linear in dO)
+    return once({gq, gk, gv, Tensor(), Tensor()}, grads, q.requires_grad() || k.requires_grad());   // (v's alone is linear in dO)
   }
 };
 
-Tensor attend_tokens(const Tensor &q, const Tensor &k, const Tensor &v, const MaybeTensor &keep_, const c10::optional<double> &scale_, int64_t stream) {
+Tensor attend_tokens(const Tensor &q, const Tensor &k, const Tensor &v, const MaybeTensor &keep_, const c10::optional<double> &scale_) {
   TORCH_CHECK_VALUE(q.dim() == 4 && k.dim() == 4 && k.sizes() == v.sizes(), "q is (B, Lq, H, D), k and v are (B, Lk, Hkv, D)");
   const int64_t B = q.size(0), H = q.size(2), D = q.size(3), Lk = k.size(1), E = k.size(2);
   TORCH_CHECK_VALUE(k.size(0) == B && k.size(3) == D && D >= 1 && D <= 128, "q, k and v share the batch and a head size of 1 to 128");
@@ -253,9 +251,9 @@ Tensor attend_tokens(const Tensor &q, const Tensor &k, const Tensor &v, const Ma
   no_forward_mode({&q, &k, &v});
   same_device(q, {&k, &v, &keep});
   if (keep.defined()) keep = (keep.scalar_type() == at::kBool || keep.scalar_type() == at::kByte ? keep : keep.ne(0)).contiguous();
-  if (wants_grad({&q, &k, &v})) return Attend::apply(q, k, v, some(keep), scale, stream);
+  if (wants_grad({&q, &k, &v})) return Attend::apply(q, k, v, some(keep), scale);
   const c10::DeviceGuard guard(q.device());
-  return attend_forward(rows_packed(q), rows_packed(k), rows_packed(v), keep, scale, Tensor(), Tensor(), stream);
+  return attend_forward(rows_packed(q), rows_packed(k), rows_packed(v), keep, scale, Tensor(), Tensor());
 }
 
 // ---- norms around a block ----------------------------------------------------------------------------------------------
@@ -264,31 +262,30 @@ struct Norm {
   Tensor residual, branch, weight, bias, post, gate, draws;
 };
 
-Tensor norm_forward(const mvr_norm_params &p, const Norm &t, Tensor &y, Tensor &z, bool training, int64_t stream) {
+Tensor norm_forward(const mvr_norm_params &p, const Norm &t, Tensor &y, Tensor &z, bool training) {
   y = at::empty(t.residual.sizes(), t.residual.options()), z = at::empty(t.branch.sizes(), t.branch.options());
   const Tensor stats = training ? at::empty({p.rows, 4}, y.options().dtype(at::kFloat)) : Tensor();
   if (p.rows)
     check(g_entry.norm(&p, t.residual.data_ptr(), t.branch.data_ptr(), t.weight.data_ptr(), ptr(t.bias), ptr(t.post), ptr(t.gate), fptr(t.draws), y.data_ptr(),
-                       z.data_ptr(), fptr(stats), stream_of(stream)),
+                       z.data_ptr(), fptr(stats), stream_of(t.residual)),
           "mvr_add_norm_tokens_forward");
   return stats;
 }
 
 struct AddNorm : public torch::autograd::Function<AddNorm> {
   static variable_list forward(AutogradContext *ctx, const Tensor &residual, const Tensor &branch, const Tensor &weight, const MaybeTensor &bias_,
-                               const MaybeTensor &post_, const MaybeTensor &gate_, const MaybeTensor &draws_, const std::string &params, int64_t stream) {
+                               const MaybeTensor &post_, const MaybeTensor &gate_, const MaybeTensor &draws_, const std::string &params) {
     const Tensor bias = or_none(bias_), post = or_none(post_), gate = or_none(gate_), draws = or_none(draws_);
     mvr_norm_params p;
     std::memcpy(&p, params.data(), sizeof(p));
     const c10::DeviceGuard guard(residual.device());
     const Norm t{packed(residual), packed(branch), packed(weight), packed(bias), packed(post), packed(gate), draws};
     Tensor y, z;
-    const Tensor stats = norm_forward(p, t, y, z, true, stream);
+    const Tensor stats = norm_forward(p, t, y, z, true);
     ctx->set_materialize_grads(false);
     // (y in 32 bits is what the backward needs; in 16 bits it would bring its rounding along, and the backward forms it again)
     ctx->save_for_backward({p.residual_type == MVR_TYPE_FLOAT ? y : t.residual, t.branch, t.weight, t.post, t.gate, draws, stats});
     ctx->saved_data["params"] = params;
-    ctx->saved_data["stream"] = stream;
     ctx->saved_data["need"] = std::vector<int64_t>{weight.requires_grad(), bias.defined() && bias.requires_grad(), post.defined() && post.requires_grad(),
                                                    gate.defined() && gate.requires_grad(),
                                                    // (weight's and bias' alone are linear in dz)
@@ -296,7 +293,7 @@ struct AddNorm : public torch::autograd::Function<AddNorm> {
     return {y, z};
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
-    variable_list none(9);
+    variable_list none(8);
     if (!grads[0].defined() && !grads[1].defined()) return none;
     const auto s = ctx->get_saved_variables();
     const Tensor &y = s[0] /* or the residual */, &branch = s[1], &weight = s[2], &post = s[3], &gate = s[4], &draws = s[5], &stats = s[6];
@@ -312,19 +309,18 @@ struct AddNorm : public torch::autograd::Function<AddNorm> {
       const size_t bytes = need[0] || need[1] || need[2] || need[3] ? g_entry.norm_bytes(&p) : 0;
       const Tensor ws = workspace(bytes, y);
       check(g_entry.norm_backward(&p, y.data_ptr(), branch.data_ptr(), weight.data_ptr(), ptr(post), ptr(gate), fptr(draws), stats.data_ptr<float>(), ptr(gy), ptr(gz),
-                                  gr.data_ptr(), gb.data_ptr(), ptr(gw), ptr(gbias), ptr(gpost), ptr(ggate), ptr(ws), bytes,
-                                  stream_of(ctx->saved_data["stream"].toInt())),
+                                  gr.data_ptr(), gb.data_ptr(), ptr(gw), ptr(gbias), ptr(gpost), ptr(ggate), ptr(ws), bytes, stream_of(y)),
             "mvr_add_norm_tokens_backward");
     } else {
       for (const Tensor *t : {&gw, &gbias, &gpost, &ggate})
         if (t->defined()) t->zero_();
     }
-    return once({gr, gb, gw, gbias, gpost, ggate, Tensor(), Tensor(), Tensor()}, grads, need[4]);
+    return once({gr, gb, gw, gbias, gpost, ggate, Tensor(), Tensor()}, grads, need[4]);
   }
 };
 
 std::vector<Tensor> add_norm_tokens(const Tensor &residual, const Tensor &branch, const Tensor &weight, const MaybeTensor &bias_, const MaybeTensor &post_,
-                                    const MaybeTensor &gate_, const MaybeTensor &draws_, double number, bool layer, double eps, int64_t stream) {
+                                    const MaybeTensor &gate_, const MaybeTensor &draws_, double number, bool layer, double eps) {
   const Tensor bias = or_none(bias_), post = or_none(post_), gate = or_none(gate_);
   Tensor draws = or_none(draws_);
   TORCH_CHECK_VALUE(residual.sizes() == branch.sizes() && residual.dim() >= 2, "residual and branch are of one shape (..., D)");
@@ -361,10 +357,10 @@ std::vector<Tensor> add_norm_tokens(const Tensor &residual, const Tensor &branch
   p.rows = rows, p.dim = (int32_t)D, p.residual_type = r, p.branch_type = b, p.param_type = type_of(weight), p.kind = layer;
   p.gate_groups = groups, p.scale_groups = draws.defined() ? draws.numel() : 0, p.scale = (float)number, p.eps = (float)eps;
   if (wants_grad({&residual, &branch, &weight, &bias, &post, &gate}))
-    return AddNorm::apply(residual, branch, weight, some(bias), some(post), some(gate), some(draws), std::string(reinterpret_cast<const char *>(&p), sizeof(p)), stream);
+    return AddNorm::apply(residual, branch, weight, some(bias), some(post), some(gate), some(draws), std::string(reinterpret_cast<const char *>(&p), sizeof(p)));
   const c10::DeviceGuard guard(residual.device());
   Tensor y, z;
-  norm_forward(p, Norm{packed(residual), packed(branch), packed(weight), packed(bias), packed(post), packed(gate), draws}, y, z, false, stream);
+  norm_forward(p, Norm{packed(residual), packed(branch), packed(weight), packed(bias), packed(post), packed(gate), draws}, y, z, false);
   return {y, z};
 }
 
@@ -372,10 +368,10 @@ std::vector<Tensor> add_norm_tokens(const Tensor &residual, const Tensor &branch
 
 TORCH_LIBRARY(mvr_tokens, m) {
   m.def("init(int[] entry_points) -> ()", init);
-  m.def("rotate(Tensor x, Tensor positions, Tensor turns, int[] sections, bool interleaved, int stream) -> Tensor");
-  m.def("attend(Tensor q, Tensor k, Tensor v, Tensor? keep, float? scale, int stream) -> Tensor");
+  m.def("rotate(Tensor x, Tensor positions, Tensor turns, int[] sections, bool interleaved) -> Tensor");
+  m.def("attend(Tensor q, Tensor k, Tensor v, Tensor? keep, float? scale) -> Tensor");
   m.def("add_norm(Tensor residual, Tensor branch, Tensor weight, Tensor? bias, Tensor? post_weight, Tensor? gate, Tensor? draws, float number, bool layer, "
-        "float eps, int stream) -> Tensor[]");
+        "float eps) -> Tensor[]");
 }
 
 // (the autograd nodes are built inside: each operator is registered for every backend key at once, as a composite)

@@ -19,11 +19,6 @@ import torch
 from torch import nn
 
 from . import _lib
-from .functional import _raw_stream
-
-
-def _stream(t):
-    return _raw_stream(t.device.index) if t.is_cuda else 0
 
 
 # ---------------------------------------------------------------------------------------------
@@ -74,7 +69,7 @@ class TokenRotary(nn.Module):
         return "sections=%s, interleaved=%s" % (self.sections, self.interleaved)
 
     def forward(self, x, positions):
-        return _lib.token_op().rotate(x, positions, self._table[0], self.sections, self.interleaved, _stream(x))
+        return _lib.token_op().rotate(x, positions, self._table[0], self.sections, self.interleaved)
 
 
 # ---------------------------------------------------------------------------------------------
@@ -89,7 +84,7 @@ def attend_tokens(q, k, v, keep=None, scale=None):
     (`draw_regularization`'s scale, viewed as (B, V)).  Of keys that are left out nothing enters the output, whatever they hold, and they get
     gradient 0; a query without any key left gets 0.  Returns (B, Lq, H, D), differentiable with respect to q, k and v: the backward recomputes
     the probabilities."""
-    return _lib.token_op().attend(q, k, v, keep, scale, _stream(q))
+    return _lib.token_op().attend(q, k, v, keep, scale)
 
 
 # ---------------------------------------------------------------------------------------------
@@ -113,4 +108,4 @@ def add_norm_tokens(residual, branch, weight, bias=None, post_weight=None, gate=
     if kind not in ("rms", "layer"):
         raise ValueError("kind is 'rms' or 'layer'")
     draws, number = (scale, 1.0) if torch.is_tensor(scale) else (None, 1.0 if scale is None else float(scale))
-    return tuple(_lib.token_op().add_norm(residual, branch, weight, bias, post_weight, gate, draws, number, kind == "layer", eps, _stream(residual)))
+    return tuple(_lib.token_op().add_norm(residual, branch, weight, bias, post_weight, gate, draws, number, kind == "layer", eps))

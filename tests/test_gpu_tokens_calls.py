@@ -56,3 +56,51 @@ def test_a_penalty_on_gradients_is_noticed():
         leaf.grad = None
         (out.float().sum() + first.float().square().sum()).backward()
         assert torch.equal(leaf.grad, first)
+
+
+def _operators(dtype=torch.bfloat16):
+    """(call, inputs): each operator as a function of tensors alone."""
+    g = _gen(92)
+    rotary = tokens.TokenRotary((4, 4), periods=(360.0, None))
+    draws = torch.tensor([[0.0, 2.0, 2.0], [2.0, 0.0, 2.0]], device=_dev())
+    keep = torch.tensor([[1, 0, 1], [0, 1, 1]], device=_dev())
+    r = lambda *s: _randn(g, *s, dtype=dtype)  # noqa: E731
+    return [(rotary, [r(2, 90, 2, 24), _randn(g, 90, 2) * 20]),
+            (lambda q, k, v: tokens.attend_tokens(q, k, v, keep=keep), [r(2, 40, 4, 64), r(2, 90, 2, 64), r(2, 90, 2, 64)]),
+            (lambda x, a, w, p: tokens.add_norm_tokens(x, a, w, post_weight=p, scale=draws)[1], [r(2, 90, 72), r(2, 90, 72), r(72), r(72)])]
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("which", range(3))
+def test_a_traced_call_runs_on_the_replays_stream(which):
+    call, inputs = _operators()[which]
+    want = call(*inputs)
+    traced = torch.jit.trace(call, tuple(inputs), check_trace=False)
+    late = torch.zeros_like(inputs[0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)   # (some 20 ms: a launch on another stream would read the zeros)
+        late.copy_(inputs[0])
+        got = traced(late, *inputs[1:])
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("which", range(3))
+def test_a_backward_called_on_another_stream(which):
+    """The gradients are computed on the forward's stream, as those of torch's operators, and handed over to the caller's."""
+    call, inputs = _operators()[which]
+    leaves = [t.requires_grad_() for t in inputs]
+    out = call(*leaves)
+    up = torch.ones_like(out)
+    want = torch.autograd.grad(out, leaves, up, retain_graph=True)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        late = torch.zeros_like(up).copy_(up)
+        got = torch.autograd.grad(out, leaves, late)
+        got = [t.clone() for t in got]
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

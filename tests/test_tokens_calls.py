@@ -45,3 +45,11 @@ def test_attention_c_abi_with_the_rest_refuses_before_any_launch():
         assert forward(rest) == 1
     assert lib.mvr_attend_tokens_backward_rest(a, p, p, p, None, p, p, None, p, p, p, p, p, 1 << 40, None) == 1
     assert lib.mvr_attend_tokens_backward_rest(a, p, p, p, None, p, p, p, p, p, p, p, None, 0, None) == 3
+
+
+def test_a_call_does_not_record_a_stream():
+    """A traced call runs on the stream that is current when it is replayed: none of the operators takes a stream's handle as a number."""
+    tokens._lib.token_op()
+    for name in ("rotate", "attend", "add_norm"):
+        schema = getattr(torch.ops.mvr_tokens, name).default._schema
+        assert not [a.name for a in schema.arguments if "stream" in a.name], schema
