@@ -63,13 +63,12 @@ class TokenRotary(nn.Module):
         for n, p in zip(sections, periods):
             turns += [(j + 1) / p if p else float(base) ** (-j / n) / (2 * math.pi) for j in range(n)]
         self.turns = tuple(turns)   # turns per unit of position, pair by pair
-        self._table = [torch.tensor(turns, dtype=torch.float64)]   # (on the host, whatever the module is moved or cast to)
 
     def extra_repr(self):
         return "sections=%s, interleaved=%s" % (self.sections, self.interleaved)
 
     def forward(self, x, positions):
-        return _lib.token_op().rotate(x, positions, self._table[0], self.sections, self.interleaved)
+        return _lib.token_op().rotate(x, positions, self.turns, self.sections, self.interleaved)
 
 
 # ---------------------------------------------------------------------------------------------

@@ -104,3 +104,110 @@ def test_a_backward_called_on_another_stream(which):
         got = [t.clone() for t in got]
     torch.cuda.current_stream().wait_stream(side)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def _step(call):
+    """Forward and backward as one function of tensors: what is traced as a training step."""
+    def step(up, *inputs):
+        leaves = [t.detach().requires_grad_() for t in inputs]
+        out = call(*leaves)
+        return (out.detach(),) + torch.autograd.grad(out, leaves, up)
+    return step
+
+
+@pytest.mark.parametrize("mode", ["real", "fake", "symbolic"])
+@pytest.mark.parametrize("which", range(3))
+def test_a_recorded_graph_computes(which, mode):
+    """make_fx's graph of a call, and of a call with its backward, gives what the call gives, on other inputs than it was recorded with."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    call, inputs = _operators()[which]
+    other = [t.flip(0) if t.dim() > 1 else t * 2 for t in inputs]
+    graph = make_fx(call, tracing_mode=mode, _allow_non_fake_inputs=True)(*inputs)
+    assert torch.equal(graph(*other), call(*other))
+    up = torch.randn_like(call(*inputs))
+    step = make_fx(_step(call), tracing_mode=mode, _allow_non_fake_inputs=True)(up, *inputs)
+    assert all(torch.equal(a, b) for a, b in zip(step(up, *other), _step(call)(up, *other)))
+    # the graph's inner operators carry gradients themselves
+    leaves = [t.detach().requires_grad_() for t in inputs]
+    want = torch.autograd.grad(call(*leaves), leaves, up)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(graph(*leaves), leaves, up), want))
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("dynamic", [False, True])
+@pytest.mark.parametrize("which", range(3))
+def test_a_compiled_call_computes(which, dynamic):
+    call, inputs = _operators()[which]
+    torch._dynamo.reset()
+    compiled = torch.compile(call, backend="aot_eager", dynamic=dynamic)
+    for args in (inputs, [t.flip(0) if t.dim() > 1 else t * 2 for t in inputs]):
+        assert torch.equal(compiled(*args), call(*args))
+        leaves = [t.detach().requires_grad_() for t in args]
+        out = compiled(*leaves)
+        up = torch.randn_like(out)
+        want = torch.autograd.grad(call(*leaves), leaves, up)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, leaves, up), want))
+
+
+def test_every_operator_is_registered_whole():
+    """torch's own check of a custom operator: schema, autograd, shapes without memory, tracing (of shapes that vary too)."""
+    ops = torch.ops.mvr_tokens
+    rotary, attend, norm = _operators()
+    need = lambda ts: [t.detach().requires_grad_() for t in ts]  # noqa: E731
+    x, pos = rotary[1]
+    pos = pos.expand(2, 90, 2).contiguous()
+    turns, sections = list(rotary[0].turns), list(rotary[0].sections)
+    q, k, v = attend[1]
+    keep = torch.tensor([[1, 0, 1], [0, 1, 1]], device=_dev()).bool()
+    r, a, w, p = norm[1]
+    draws = torch.tensor([[0.0, 2.0, 2.0], [2.0, 0.0, 2.0]], device=_dev())
+    with torch.no_grad():
+        out, rest, lse = ops.attend_training(q, k, v, keep, 0.125)
+        stats = ops.add_norm_training(r, a, w, None, p, None, draws, 1.0, False, 1e-6)[2]
+    for op, args in ((ops.rotate_forward, (*need((x, pos)), turns, sections, False)), (ops.rotate_backward, (x, x, pos, turns, sections, False)),
+                     (ops.attend_forward, (*need((q, k, v)), keep, 0.125)), (ops.attend_training, (q, k, v, keep, 0.125)),
+                     (ops.attend_backward, (q, q, k, v, keep, out, rest, lse, 0.125)),
+                     (ops.add_norm_forward, (*need((r, a, w)), None, *need((p,)), None, draws, 1.0, False, 1e-6)),
+                     (ops.add_norm_training, (r, a, w, None, p, None, draws, 1.0, False, 1e-6)),
+                     (ops.add_norm_backward, (r, None, r, a, w, p, None, draws, stats, [1, 0, 1, 0], 1.0, False, 1e-6))):
+        torch.library.opcheck(op.default, args)
+
+
+def test_inner_operators_refuse_what_does_not_fit():
+    """A graph that was edited, or a call around mvtn_amd.tokens: every way to the kernels checks shapes, types and devices."""
+    ops = torch.ops.mvr_tokens
+    (_, (x, pos)), (_, (q, k, v)), (_, (r, a, w, p)) = _operators()
+    tokens._lib.token_op()
+    pos = pos.expand(2, 90, 2).contiguous()
+    keep = torch.ones(2, 3, device=_dev(), dtype=torch.bool)
+    out, rest, lse = ops.attend_training(q, k, v, keep, 0.125)
+    stats = ops.add_norm_training(r, a, w, None, p, None, None, 1.0, False, 1e-6)[2]
+    for op, args in ((ops.rotate_forward, (x, pos[:1], [0.1] * 8, [4, 4], False)), (ops.rotate_forward, (x, pos.double(), [0.1] * 8, [4, 4], False)),
+                     (ops.rotate_forward, (x, pos, [0.1] * 7, [4, 4], False)), (ops.rotate_forward, (x, pos, [0.1] * 8, [4, 4, 0], False)),
+                     (ops.rotate_backward, (x, x[:1], pos, [0.1] * 8, [4, 4], False)), (ops.attend_forward, (q, k, v, keep.float(), 0.125)),
+                     (ops.attend_training, (q, k, v[:, :-1], keep, 0.125)), (ops.attend_backward, (q[:, :-1], q, k, v, keep, out, rest, lse, 0.125)),
+                     (ops.attend_backward, (q, q, k, v, keep, out, rest[:0], lse, 0.125)), (ops.attend_backward, (q, q, k, v, keep, out, rest, lse[..., :-1], 0.125)),
+                     (ops.attend_backward, (q, q, k, v, keep, out.float(), rest, lse, 0.125)),
+                     (ops.add_norm_training, (r, a, w, None, p, None, torch.ones(2, device=_dev(), dtype=torch.float64), 1.0, False, 1e-6)),
+                     (ops.add_norm_backward, (r, None, r, a, w, p, None, None, stats[:-1], [1, 0, 1, 0], 1.0, False, 1e-6)),
+                     (ops.add_norm_backward, (None, None, r, a, w, p, None, None, stats, [1, 0, 1, 0], 1.0, False, 1e-6)),
+                     (ops.add_norm_backward, (r, None, r, a, w, None, None, None, stats, [1, 0, 1, 0], 1.0, False, 1e-6)),
+                     (ops.add_norm_backward, (r, None, r, a, w, p, None, None, stats, [1, 0], 1.0, False, 1e-6))):
+        with pytest.raises(ValueError):
+            op(*args)
+    with pytest.raises(RuntimeError, match="one GPU|on the GPU"):
+        ops.rotate_forward(x, pos.cpu(), [0.1] * 8, [4, 4], False)
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("which", range(3))
+def test_vmap_and_function_transforms(which):
+    """vmap runs call by call; grad through functorch is refused, and not wrong."""
+    call, inputs = _operators()[which]
+    stacked = torch.stack([inputs[0], inputs[0].flip(0)])
+    got = torch.func.vmap(lambda t: call(t, *inputs[1:]))(stacked)
+    assert torch.equal(got, torch.stack([call(t, *inputs[1:]) for t in stacked]))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda t: call(t, *inputs[1:]).float().sum())(inputs[0])
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(lambda t: call(t, *inputs[1:]), (inputs[0],), (inputs[0],))

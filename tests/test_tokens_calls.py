@@ -53,3 +53,41 @@ def test_a_call_does_not_record_a_stream():
     for name in ("rotate", "attend", "add_norm"):
         schema = getattr(torch.ops.mvr_tokens, name).default._schema
         assert not [a.name for a in schema.arguments if "stream" in a.name], schema
+
+
+def _on_fake_gpu():
+    """(call, inputs) of each operator on tensors that have shapes and a device and no memory."""
+    rotary = tokens.TokenRotary((4, 4), periods=(360.0, None))
+    e = lambda *s, dtype=torch.bfloat16: torch.empty(*s, dtype=dtype, device="cuda")  # noqa: E731
+    draws, keep = e(2, 3, dtype=torch.float32), e(2, 3, dtype=torch.float32)
+    return [(rotary, [e(2, 90, 2, 24), e(90, 2, dtype=torch.float32)], [(2, 90, 2, 24)]),
+            (lambda q, k, v: tokens.attend_tokens(q, k, v, keep=keep), [e(2, 40, 4, 64).transpose(1, 2).contiguous().transpose(1, 2), e(2, 90, 2, 64), e(2, 90, 2, 64)], [(2, 40, 4, 64)]),
+            (lambda x, a, w, gate: tokens.add_norm_tokens(x, a, w, gate=gate, scale=draws), [e(2, 90, 72, dtype=torch.float32), e(2, 90, 72), e(72), e(2, 72)], [(2, 90, 72)] * 2)]
+
+
+@pytest.mark.parametrize("which", range(3))
+def test_shapes_without_memory(which):
+    """Under a tracer of shapes the operators give tensors of the right shape, type and layout; and what does not fit is refused as ever."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        call, inputs, shapes = _on_fake_gpu()[which]
+        out = call(*inputs)
+        out = out if isinstance(out, tuple) else (out,)
+        assert [tuple(t.shape) for t in out] == shapes and all(t.is_contiguous() and t.device.type == "cuda" for t in out)
+        assert [t.dtype for t in out] == ([torch.float32, torch.bfloat16] if which == 2 else [torch.bfloat16])
+        out = call(*[t.requires_grad_() for t in inputs])
+        assert all(t.requires_grad for t in (out if isinstance(out, tuple) else (out,)))
+        with pytest.raises(ValueError):
+            call(inputs[0][..., :15], *inputs[1:])
+
+
+@pytest.mark.parametrize("which", range(3))
+def test_a_graph_of_a_call_holds_the_operator(which):
+    """What a tracer below autograd records is the operator, not the allocation of its result alone."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        call, inputs, _ = _on_fake_gpu()[which]
+        graph = make_fx(call)(*inputs).graph
+    names = [str(n.target) for n in graph.nodes if n.op == "call_function"]
+    assert [n for n in names if n.startswith("mvr_tokens.")] == [("mvr_tokens.rotate_forward.default", "mvr_tokens.attend_forward.default", "mvr_tokens.add_norm_forward.default")[which]], names
