@@ -334,7 +334,7 @@ __global__ __launch_bounds__(WAVES > 1 ? 64 * WAVES : kBlock) void k_add_norm(No
   bool dropped = false;
   const auto fetch = [&](unsigned row) {
     s = a.scale ? a.scale[row / scale_rows] : a.s;
-    dropped = a.scale && s == 0.0f;   // a dropped view's branch is not read: whatever it holds stays out
+    dropped = s == 0.0f;   // a dropped view's branch is not read: whatever it holds stays out
     const TR *rp = (const TR *)a.residual + (int64_t)row * a.D;
     const TB *bp = (const TB *)a.branch + (int64_t)row * a.D;
 #pragma unroll
@@ -423,7 +423,7 @@ __global__ __launch_bounds__(WAVES > 1 ? 64 * WAVES : kBlock) void k_add_norm_ba
   float4 stats;
   const auto fetch = [&](unsigned row) {
     s = a.scale ? a.scale[row / scale_rows] : a.s;
-    dropped = a.scale && s == 0.0f;
+    dropped = s == 0.0f;
     stats = *reinterpret_cast<const float4 *>(a.stats + (int64_t)row * 4);
     const int64_t base = (int64_t)row * a.D;
 #pragma unroll

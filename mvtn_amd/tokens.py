@@ -103,7 +103,7 @@ def add_norm_tokens(residual, branch, weight, bias=None, post_weight=None, gate=
     residual, branch: one shape (..., D); float32, float16 or bfloat16 alike, or a float32 residual with a 16-bit branch.  weight, bias,
     post_weight: (D,).  gate: (D,), or one row per leading index: (B, D) or (B, 1, D) with residual (B, L, D).  The four share one type.
     scale: a number, or float32 draws for equal runs of rows in memory order — `draw_regularization`'s scale, one per view: a row whose
-    draw is 0 keeps its residual, its branch is not read and gets gradient 0.  Differentiable with respect to everything but scale."""
+    scale is 0 keeps its residual, its branch is not read and gets gradient 0.  Differentiable with respect to everything but scale."""
     if kind not in ("rms", "layer"):
         raise ValueError("kind is 'rms' or 'layer'")
     draws, number = (scale, 1.0) if torch.is_tensor(scale) else (None, 1.0 if scale is None else float(scale))

@@ -211,3 +211,26 @@ def test_vmap_and_function_transforms(which):
         torch.func.grad(lambda t: call(t, *inputs[1:]).float().sum())(inputs[0])
     with pytest.raises(RuntimeError, match="forward-mode"):
         torch.func.jvp(lambda t: call(t, *inputs[1:]), (inputs[0],), (inputs[0],))
+
+
+def _norm_call(t, scale, kind="rms"):
+    return tokens.add_norm_tokens(t["residual"], t["branch"], t["weight"], post_weight=t.get("post"), gate=t.get("gate"), scale=scale, kind=kind)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("D,post", [(72, False), (72, True), (1500, True)])
+def test_a_scale_of_zero_as_a_number_leaves_the_branch_out(dtype, D, post):
+    """scale=0.0 for all rows is what draws of 0 for all of them are: the residual stays, whatever the branch holds."""
+    g = _gen(93)
+    t = {"residual": _randn(g, 2, 6, D, dtype=dtype), "branch": _randn(g, 2, 6, D, dtype=dtype), "weight": _randn(g, D, dtype=dtype), "gate": _randn(g, 2, D, dtype=dtype)}
+    if post:
+        t["post"] = _randn(g, D, dtype=dtype)
+    t["branch"][0, 1, 3], t["branch"][1, 0, 2] = math.nan, math.inf
+    results = []
+    for scale in (0.0, torch.zeros(2, device=_dev())):
+        leaves = {k: v.detach().requires_grad_() for k, v in t.items()}
+        y, z = _norm_call(leaves, scale)
+        grads = torch.autograd.grad((y, z), list(leaves.values()), (torch.ones_like(y), torch.ones_like(z)))
+        results.append([y.detach(), z.detach()] + list(grads))
+        assert torch.equal(y, t["residual"]) and not grads[1].any() and all(torch.isfinite(x).all() for x in results[-1])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
