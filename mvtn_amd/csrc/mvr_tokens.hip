@@ -480,9 +480,9 @@ __global__ __launch_bounds__(WAVES > 1 ? 64 * WAVES : kBlock) void k_add_norm_ba
       for (int k = 0; k < kV; ++k) {
         t[j][k] += st.y * (g[j][k] - m1 - y[j][k] * m0);          // dyt
         const float hat = n[j][k];
-        const float u = k < left[j] ? s0 * t[j][k] : 0.0f;
+        const float u = !gone && k < left[j] ? s0 * t[j][k] : 0.0f;   // (0 times an infinite dyt is not 0)
         dg[j][k] += u * po[k] * hat;
-        const float dn = gone ? 0.0f : u * ga[k];
+        const float dn = u * ga[k];
         dp[j][k] += dn * hat;
         g[j][k] = dn * po[k];
         d[0] += g[j][k] * hat;

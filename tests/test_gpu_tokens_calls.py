@@ -234,3 +234,24 @@ def test_a_scale_of_zero_as_a_number_leaves_the_branch_out(dtype, D, post):
         results.append([y.detach(), z.detach()] + list(grads))
         assert torch.equal(y, t["residual"]) and not grads[1].any() and all(torch.isfinite(x).all() for x in results[-1])
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("D", [72, 1500])
+def test_a_dropped_rows_infinite_gradient_stays_out_of_the_gates(dtype, D):
+    """A row whose scale is 0 has no part in n: gate and post_weight get from it nothing, whatever comes down its residual."""
+    g = _gen(94)
+    t = {"residual": _randn(g, 2, 8, D, dtype=dtype), "branch": _randn(g, 2, 8, D, dtype=dtype), "weight": _randn(g, D, dtype=dtype), "gate": _randn(g, 2, D, dtype=dtype),
+         "post": _randn(g, D, dtype=dtype)}
+    draws = torch.tensor([[0.0, 2.0], [2.0, 2.0]], device=_dev())
+    dy, dz = _randn(g, 2, 8, D, dtype=dtype), _randn(g, 2, 8, D, dtype=dtype)
+    results = []
+    for bad in (0.0, math.inf):
+        leaves = {k: v.detach().requires_grad_() for k, v in t.items()}
+        up = dy.clone()
+        up[0, 1, 5] = bad
+        out = _norm_call(leaves, draws)
+        results.append(dict(zip(leaves, torch.autograd.grad(out, list(leaves.values()), (up, dz)))))
+    clean, got = results
+    assert torch.isinf(got["residual"][0, 1, 5]) and not got["branch"][0, :4].any()
+    assert all(torch.equal(got[k], clean[k]) for k in ("branch", "gate", "post", "weight"))
