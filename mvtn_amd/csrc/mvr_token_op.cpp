@@ -265,7 +265,9 @@ void check_attend(const Tensor &q, const Tensor &k, const Tensor &v, const Tenso
   TORCH_CHECK_VALUE(in_32_bits(q) && in_32_bits(k), "every size of q, k and v must be below 2^31");
   TORCH_CHECK_VALUE((float)scale > 0 && std::isfinite((float)scale), "scale must be positive and finite, in 32 bits too");
   if (keep.defined()) {
-    TORCH_CHECK_VALUE(keep.dim() == 2 && len(keep, 0) == B && len(keep, 1) >= 1 && Lk % len(keep, 1) == 0, "keep is (B, G) with G a divisor of the ", Lk, " keys");
+    const int64_t groups = keep.dim() == 2 ? len(keep, 1) : 0;
+    // (one entry per key of no keys: none)
+    TORCH_CHECK_VALUE(keep.dim() == 2 && len(keep, 0) == B && (groups >= 1 ? Lk % groups == 0 : Lk == 0), "keep is (B, G) with G a divisor of the ", Lk, " keys");
     TORCH_CHECK_VALUE(!keep.requires_grad(), "keep is a mask: it gets no gradient");
   }
 }
@@ -425,7 +427,7 @@ mvr_norm_params check_norm(const Tensor &residual, const Tensor &branch, const T
     TORCH_CHECK_VALUE(!draws.requires_grad(), "scale holds draws: it gets no gradient (put what is learned into gate)");
     count = 1;
     for (int64_t k = 0; k < draws.dim(); ++k) count *= len(draws, k);
-    TORCH_CHECK_VALUE(count >= 1 && rows % count == 0, "scale has ", count, " draws, which do not divide the ", rows, " rows");
+    TORCH_CHECK_VALUE(count >= 1 ? rows % count == 0 : rows == 0, "scale has ", count, " draws, which do not divide the ", rows, " rows");
   }
   mvr_norm_params p;
   std::memset(&p, 0, sizeof(p));

@@ -255,3 +255,19 @@ def test_a_dropped_rows_infinite_gradient_stays_out_of_the_gates(dtype, D):
     clean, got = results
     assert torch.isinf(got["residual"][0, 1, 5]) and not got["branch"][0, :4].any()
     assert all(torch.equal(got[k], clean[k]) for k in ("branch", "gate", "post", "weight"))
+
+
+def test_a_last_batch_without_objects():
+    """The draws of no objects, the mask of no keys: empty results and zero gradients, as without them."""
+    g = _gen(95)
+    w = _randn(g, 8).requires_grad_()
+    x, a = (torch.zeros(0, 12, 8, device=_dev(), requires_grad=True) for _ in range(2))
+    gate = torch.zeros(0, 8, device=_dev(), requires_grad=True)
+    y, z = tokens.add_norm_tokens(x, a, w, post_weight=w, gate=gate, scale=torch.zeros(0, 3, device=_dev()))
+    assert y.shape == x.shape and z.shape == x.shape
+    gx, ga, gg, gw = torch.autograd.grad((y, z), (x, a, gate, w), (y.detach(), z.detach()))
+    assert gx.shape == x.shape and ga.shape == x.shape and gg.shape == gate.shape and not gw.any()
+    h = lambda *s: torch.ones(*s, dtype=torch.float16, device=_dev())  # noqa: E731
+    for B, Lq, Lk, keep in ((0, 4, 6, (0, 3)), (2, 4, 0, (2, 0)), (2, 4, 0, (2, 5)), (0, 4, 0, (0, 0))):
+        got = _attention(h(B, Lq, 2, 16), h(B, Lk, 2, 16), h(B, Lk, 2, 16), h(B, Lq, 2, 16), torch.zeros(*keep, device=_dev()))
+        assert [tuple(t.shape) for t in got] == [(B, Lq, 2, 16)] * 2 + [(B, Lk, 2, 16)] * 2 and not any(t.any() for t in got)

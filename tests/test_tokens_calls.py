@@ -91,3 +91,16 @@ def test_a_graph_of_a_call_holds_the_operator(which):
         graph = make_fx(call)(*inputs).graph
     names = [str(n.target) for n in graph.nodes if n.op == "call_function"]
     assert [n for n in names if n.startswith("mvr_tokens.")] == [("mvr_tokens.rotate_forward.default", "mvr_tokens.attend_forward.default", "mvr_tokens.add_norm_forward.default")[which]], names
+
+
+def test_empty_masks_and_draws_only_for_empty_tensors():
+    h = lambda *s: torch.zeros(*s, dtype=torch.float16)  # noqa: E731
+    x, w = torch.zeros(0, 6, 8), torch.zeros(8)
+    with pytest.raises(RuntimeError, match="GPU"):   # (nothing wrong with the arguments)
+        tokens.attend_tokens(h(2, 3, 2, 8), h(2, 0, 2, 8), h(2, 0, 2, 8), keep=torch.zeros(2, 0))
+    with pytest.raises(RuntimeError, match="GPU"):
+        tokens.add_norm_tokens(x, x, w, scale=torch.zeros(0, 3))
+    with pytest.raises(ValueError):
+        tokens.attend_tokens(h(2, 3, 2, 8), h(2, 6, 2, 8), h(2, 6, 2, 8), keep=torch.zeros(2, 0))
+    with pytest.raises(ValueError):
+        tokens.add_norm_tokens(torch.zeros(2, 6, 8), torch.zeros(2, 6, 8), w, scale=torch.zeros(0, 3))
