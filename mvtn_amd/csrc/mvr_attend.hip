@@ -50,13 +50,15 @@ struct AttArgs {
   void *rest;                    // what out's rounding left, in its type and layout; or null
   float *lse;                    // (B, heads, queries): log2 of the sum of exp2(scale log2(e) q k); +inf for a row without keys
   float *delta;                  // the same shape
-  float *part, *part_lse;        // splits over the keys: (splits, B kv_heads rows, D) and (splits, B kv_heads rows)
+  float *part, *part_lse;        // splits over the keys: (splits, B kv_heads rows, D) and (splits, B kv_heads rows); over the rows: (row_splits, 2, B keys kv_heads, D)
   int64_t qs[3], ks[3], vs[3], gs[3];
   int32_t B, Lq, Lk, H, E, G, D;   // E: kv heads, G: heads of a group
   int32_t groups, per;           // keep: (B, groups), `per` keys each
   int32_t rows;                  // G * Lq
   int32_t tiles, splits, split_tiles, col_tiles;
+  int32_t row_splits, row_split_tiles;   // of the tiles of rows that dK and dV walk
   int32_t wide;                  // two columns of 32 queries a wave
+  int32_t rows_whole;            // whole, and a group's heads of fewer queries than a tile holds do not share tiles
   int32_t whole;                 // D a multiple of 8 and a tile's rows within 32-bit offsets: tiles are loaded in whole chunks
   int64_t work;                  // workgroups with something to do
   float c, scale;                // scale log2(e)
@@ -737,6 +739,12 @@ __global__ __launch_bounds__(kBlock) void k_attend_dq_join(AttArgs a) {
 // Heads above 64: a column of 16 keys a wave on v_mfma_f32_16x16x32, whose two sums of 16 x D leave the registers for two waves a SIMD, where 32
 // keys of 128 fill all of one.  A lane's scores are rows 16 b + 4 (lane / 16) + 0..3 of a sub-tile of 32 (b = 0, 1) of ONE key, which is the order
 // that the next product's operands take the rows in.
+//
+// Few keys: the rows are dealt to several workgroups, as the keys are in the other kernels, and their parts of dK and dV, in 32 bits, are added
+// up by k_attend_dkv_join.  4000 queries, 4 heads of 128 on one, forward and gradients, us without and with: over 12 keys (where one workgroup walked 250
+// tiles) 569 / 84, over 4000 keys 590 / 248.
+
+__device__ __forceinline__ int64_t dkv_size(const AttArgs &a) { return (int64_t)a.B * a.Lk * a.E * a.D; }
 
 template <typename T, int DP, bool WHOLE, bool FINE>
 __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv16(AttArgs a) {
@@ -745,8 +753,10 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv16(AttArgs a) {
   constexpr int kSize = Layout<DP>::kSize;
   __shared__ __attribute__((aligned(256))) T tiles[2][2 * kSize];   // two buffers of a tile of q and a tile of dO
   __shared__ __attribute__((aligned(16))) float stats[2][2][kTile];   // their lse and -delta
-  const int64_t item = work_item(a.work);
+  int64_t item = work_item(a.work);
   if (item >= a.work) return;
+  const int split = (int)(item % a.row_splits);
+  item /= a.row_splits;
   const int ct = (int)(item % a.col_tiles);
   const int64_t be = item / a.col_tiles;
   const int b = (int)(be / a.E), e = (int)(be - (int64_t)b * a.E);
@@ -770,10 +780,12 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv16(AttArgs a) {
   Stage<T, DP> staged;
   float lse = 0.0f, delta = 0.0f;
   float times = power_of_2((int)kStart);   // what this column's dS and dk are multiplied by (kNarrow)
-  const int n = !__syncthreads_or(on) ? 0 : WHOLE ? a.G * ((a.Lq + kTile - 1) / kTile) : (a.rows + kTile - 1) / kTile;   // (no kept key here: zeros)
+  const int head_tiles = (a.Lq + kTile - 1) / kTile, all_tiles = WHOLE ? a.G * head_tiles : (a.rows + kTile - 1) / kTile;
+  const int first = split * a.row_split_tiles, end = first + a.row_split_tiles < all_tiles ? first + a.row_split_tiles : all_tiles;
+  const int n = __syncthreads_or(on) ? end : first;   // (no kept key here: zeros)
   // as in walk_tiles: a tile of q beside the first half of the work, a tile of dO beside the second
   // the tile to load: with WHOLE from row i0 of head g0 (a head's last tile ends with it), else the rows from tile * kTile of the group's list
-  int g0 = 0, i0 = 0;
+  int g0 = WHOLE ? first / head_tiles : 0, i0 = WHOLE ? (first - g0 * head_tiles) * kTile : 0;
   const auto load = [&](int which, int tile) {
     const T *base = which ? gb : qb;
     const int64_t stride = which ? a.gs[1] : a.qs[1], head = which ? a.gs[2] : a.qs[2];
@@ -798,16 +810,16 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv16(AttArgs a) {
     staged.store(tiles[buffer] + which * kSize, ~0ull);
     if (which == 0 && threadIdx.x < kTile) stats[buffer][0][threadIdx.x] = lse - kLiftP<T>, stats[buffer][1][threadIdx.x] = -delta;
   };
-  if (n) {
-    load(0, 0);
+  if (first < n) {
+    load(0, first);
     store(0, 0);
-    load(1, 0);
+    load(1, first);
     store(1, 0);
   }
   loads_done();
   lds_barrier();
-  for (int tile = 0; tile < n; ++tile) {
-    const int buffer = tile & 1;
+  for (int tile = first; tile < n; ++tile) {
+    const int buffer = (tile - first) & 1;
     const R r = reader.at(buffer);
     if (tile + 1 < n) load(0, tile + 1);
 #pragma unroll
@@ -893,14 +905,21 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv16(AttArgs a) {
     for (int d = 0; d < DP / 16; ++d) dk[d] = dv[d] = 0.0f;
   }
   const int64_t to = (((int64_t)b * a.Lk + key) * a.E + e) * a.D;
-  const float dv_by = kNarrow<T> ? power_of_2(-(int)kLiftP<T>) : 1.0f, dk_by = kNarrow<T> ? a.scale * dv_by / times : a.scale;
+  const float scale = a.row_splits > 1 ? 1.0f : a.scale;   // (parts are scaled where they are added up)
+  const float dv_by = kNarrow<T> ? power_of_2(-(int)kLiftP<T>) : 1.0f, dk_by = kNarrow<T> ? scale * dv_by / times : scale;
+  float *part = a.part + split * 2 * dkv_size(a) + to;
 #pragma unroll
   for (int d = 0; d < DP / 16; ++d) {
     const int at = 16 * d + 4 * (lane >> 4);
     const float x[4] = {dk[d][0] * dk_by, dk[d][1] * dk_by, dk[d][2] * dk_by, dk[d][3] * dk_by};
     const float y[4] = {dv[d][0] * dv_by, dv[d][1] * dv_by, dv[d][2] * dv_by, dv[d][3] * dv_by};
-    store_n<4>((T *)a.dk + to + at, a.D - at, x);
-    store_n<4>((T *)a.dv + to + at, a.D - at, y);
+    if (a.row_splits > 1) {
+      store_n<4>(part + at, a.D - at, x);
+      store_n<4>(part + dkv_size(a) + at, a.D - at, y);
+    } else {
+      store_n<4>((T *)a.dk + to + at, a.D - at, x);
+      store_n<4>((T *)a.dv + to + at, a.D - at, y);
+    }
   }
 }
 
@@ -911,8 +930,10 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv32(AttArgs a) {
   constexpr int kSize = Layout<DP>::kSize;
   __shared__ __attribute__((aligned(256))) T tiles[2][2 * kSize];   // two buffers of a tile of q and a tile of dO
   __shared__ __attribute__((aligned(16))) float stats[2][2][kTile];   // their lse and -delta
-  const int64_t item = work_item(a.work);
+  int64_t item = work_item(a.work);
   if (item >= a.work) return;
+  const int split = (int)(item % a.row_splits);
+  item /= a.row_splits;
   const int ct = (int)(item % a.col_tiles);
   const int64_t be = item / a.col_tiles;
   const int b = (int)(be / a.E), e = (int)(be - (int64_t)b * a.E);
@@ -938,10 +959,12 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv32(AttArgs a) {
   const Reader<DP> reader = Reader<DP>::wide(tiles);
   float lse = 0.0f, delta = 0.0f;
   float times = power_of_2((int)kStart);   // what this column's dS and dk are multiplied by (kNarrow)
-  const int n = !__syncthreads_or(on) ? 0 : WHOLE ? a.G * ((a.Lq + kTile - 1) / kTile) : (a.rows + kTile - 1) / kTile;   // (no kept key here: zeros)
+  const int head_tiles = (a.Lq + kTile - 1) / kTile, all_tiles = WHOLE ? a.G * head_tiles : (a.rows + kTile - 1) / kTile;
+  const int first = split * a.row_split_tiles, end = first + a.row_split_tiles < all_tiles ? first + a.row_split_tiles : all_tiles;
+  const int n = __syncthreads_or(on) ? end : first;   // (no kept key here: zeros)
   // as in walk_tiles: a tile of q beside the first half of the work, a tile of dO beside the second
   // the tile to load: with WHOLE from row i0 of head g0 (a head's last tile ends with it), else the rows from tile * kTile of the group's list
-  int g0 = 0, i0 = 0;
+  int g0 = WHOLE ? first / head_tiles : 0, i0 = WHOLE ? (first - g0 * head_tiles) * kTile : 0;
   const auto load = [&](int which, int tile) {
     const T *base = which ? gb : qb;
     const int64_t stride = which ? a.gs[1] : a.qs[1], head = which ? a.gs[2] : a.qs[2];
@@ -966,16 +989,16 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv32(AttArgs a) {
     staged.store(tiles[buffer] + which * kSize, ~0ull);
     if (which == 0 && threadIdx.x < kTile) stats[buffer][0][threadIdx.x] = lse - kLiftP<T>, stats[buffer][1][threadIdx.x] = -delta;
   };
-  if (n) {
-    load(0, 0);
+  if (first < n) {
+    load(0, first);
     store(0, 0);
-    load(1, 0);
+    load(1, first);
     store(1, 0);
   }
   loads_done();
   lds_barrier();
-  for (int tile = 0; tile < n; ++tile) {
-    const int buffer = tile & 1;
+  for (int tile = first; tile < n; ++tile) {
+    const int buffer = (tile - first) & 1;
     const Reader<DP> r = reader.at(buffer);
     if (tile + 1 < n) load(0, tile + 1);
     V8 qf[DP / 16], gf[DP / 16], c[2][DP / 32];
@@ -1054,12 +1077,38 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dkv32(AttArgs a) {
     for (int d = 0; d < DP / 32; ++d) dk[d] = dv[d] = 0.0f;
   }
   const int64_t to = (((int64_t)b * a.Lk + key) * a.E + e) * a.D;
-  const float dv_by = kNarrow<T> ? power_of_2(-(int)kLiftP<T>) : 1.0f, dk_by = kNarrow<T> ? a.scale * dv_by / times : a.scale;
-  store_column<T, DP>((T *)a.dk + to, a.D, dk, dk_by);
-  store_column<T, DP>((T *)a.dv + to, a.D, dv, dv_by);
+  const float scale = a.row_splits > 1 ? 1.0f : a.scale;   // (as above)
+  const float dv_by = kNarrow<T> ? power_of_2(-(int)kLiftP<T>) : 1.0f, dk_by = kNarrow<T> ? scale * dv_by / times : scale;
+  if (a.row_splits > 1) {
+    float *part = a.part + split * 2 * dkv_size(a) + to;
+    store_column<float, DP>(part, a.D, dk, dk_by);
+    store_column<float, DP>(part + dkv_size(a), a.D, dv, dv_by);
+  } else {
+    store_column<T, DP>((T *)a.dk + to, a.D, dk, dk_by);
+    store_column<T, DP>((T *)a.dv + to, a.D, dv, dv_by);
+  }
+}
+
+// one wave per key and head: the parts of the rows' splits, in order
+template <typename T>
+__global__ __launch_bounds__(kBlock) void k_attend_dkv_join(AttArgs a) {
+  const int64_t lines = (int64_t)a.B * a.Lk * a.E, line = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
+  if (line >= lines) return;
+  const int lane = threadIdx.x & 63;
+  for (int k = 0; k < 2; ++k) {
+    const int64_t at = line * a.D + lane + 64 * k;
+    if (lane + 64 * k >= a.D) break;
+    float x = 0.0f, y = 0.0f;
+    for (int s = 0; s < a.row_splits; ++s) x += a.part[2 * s * dkv_size(a) + at], y += a.part[(2 * s + 1) * dkv_size(a) + at];
+    ((T *)a.dk)[at] = (T)(x * a.scale);
+    ((T *)a.dv)[at] = (T)y;
+  }
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------
+
+// keys of a workgroup of dK and dV
+constexpr int dkv_keys(int D) { return D <= 64 ? 32 * kWaves : 16 * kWaves; }
 
 int att_args(AttArgs &a, const mvr_attend_params *p) {
   if (!p) return bad("mvr_attend_tokens: params must be given");
@@ -1091,13 +1140,26 @@ int att_args(AttArgs &a, const mvr_attend_params *p) {
   a.splits = splits < 2 ? 1 : (int32_t)splits;
   a.split_tiles = (a.tiles + a.splits - 1) / a.splits;
   a.splits = (a.tiles + a.split_tiles - 1) / a.split_tiles;
+  // few keys: the same for the rows that dK and dV walk
+  a.rows_whole = a.whole && (a.G == 1 || a.Lq >= kTile);
+  const int64_t row_tiles = a.rows_whole ? (int64_t)a.G * ((a.Lq + kTile - 1) / kTile) : (rows + kTile - 1) / kTile;
+  const int64_t key_blocks = (a.Lk + dkv_keys(a.D) - 1) / dkv_keys(a.D) * a.B * a.E;
+  splits = 512 / key_blocks, most = row_tiles / 4;
+  splits = splits > most ? most : splits;
+  a.row_splits = splits < 2 ? 1 : (int32_t)splits;
+  a.row_split_tiles = (int32_t)((row_tiles + a.row_splits - 1) / a.row_splits);
+  a.row_splits = (int32_t)((row_tiles + a.row_split_tiles - 1) / a.row_split_tiles);
   return MVR_OK;
 }
 
 size_t lines(const AttArgs &a) { return (size_t)a.B * a.E * a.rows; }
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 size_t forward_bytes(const AttArgs &a) { return a.splits > 1 ? align256(lines(a) * a.splits * a.D * 4) + align256(lines(a) * a.splits * 4) : 0; }
-size_t backward_bytes(const AttArgs &a) { return align256(lines(a) * 4) + (a.splits > 1 ? align256(lines(a) * a.splits * a.D * 4) : 0); }
+// delta, and the parts of dQ or, behind them in time, of dK and dV
+size_t backward_bytes(const AttArgs &a) {
+  const size_t dq = a.splits > 1 ? lines(a) * a.splits * a.D * 4 : 0, dkv = a.row_splits > 1 ? (size_t)a.B * a.Lk * a.E * a.D * a.row_splits * 2 * 4 : 0;
+  return align256(lines(a) * 4) + align256(dq > dkv ? dq : dkv);
+}
 
 // workgroups of `per` columns each, a multiple of 8 for work_item
 bool grid_of(AttArgs &a, int64_t columns, int per, int splits, unsigned &blocks) {
@@ -1151,10 +1213,8 @@ int launch_backward(AttArgs a, hipStream_t st) {
     hipLaunchKernelGGL((k_attend_dq_join<T>), dim3((unsigned)((lines(a) + kWaves - 1) / kWaves)), dim3(kBlock), 0, st, a);
     if (int rc = launched("k_attend_dq_join")) return rc;
   }
-  // a group's heads of fewer queries than a tile holds share tiles
-  const bool whole = a.whole && (a.G == 1 || a.Lq >= kTile);
-  constexpr int kKeys = DP <= 64 ? 32 * kWaves : 16 * kWaves;
-  if (!grid_of(a, a.Lk, kKeys, 1, n)) return bad("mvr_attend_tokens_backward: too many workgroups");
+  const bool whole = a.rows_whole;
+  if (!grid_of(a, a.Lk, dkv_keys(DP), a.row_splits, n)) return bad("mvr_attend_tokens_backward: too many workgroups");
   const dim3 g(n), blk(kBlock);
 #define MVR_ATT_KEYS(kernel)                                                                \
   do {                                                                                      \
@@ -1166,7 +1226,10 @@ int launch_backward(AttArgs a, hipStream_t st) {
   if constexpr (DP <= 64) MVR_ATT_KEYS(k_attend_dkv32);
   else MVR_ATT_KEYS(k_attend_dkv16);
 #undef MVR_ATT_KEYS
-  return launched("k_attend_dkv");
+  if (int rc = launched("k_attend_dkv")) return rc;
+  if (a.row_splits == 1) return MVR_OK;
+  hipLaunchKernelGGL((k_attend_dkv_join<T>), dim3((unsigned)(((int64_t)a.B * a.Lk * a.E + kWaves - 1) / kWaves)), dim3(kBlock), 0, st, a);
+  return launched("k_attend_dkv_join");
 }
 
 // heads are padded with zeros to the next of 32, 64, 96, 128

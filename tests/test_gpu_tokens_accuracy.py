@@ -34,7 +34,11 @@ def _sizes(q, k, v, do, scale, keep=None, stored_out=False):
             p = torch.softmax(Q @ K.T * scale, -1)
             o = p @ V
             ds = p * (G @ V.T - (G * o).sum(-1, keepdim=True))
-            delta = ds.square().sum(-1, keepdim=True)
+            # dP and delta are 32-bit sums of D products: D roundings, each of 2^-24 of a partial sum, whose square is in the mean at most that of the whole,
+            # the products' squares added up (four times that here).  Nothing beside the rest, but where one key has all of P dP - delta is 0
+            r = 4 * D * 2.0 ** -48 / f
+            ds2 = ds.square() + p.square() * r * (G.square() @ V.square().T)
+            delta = ds.square().sum(-1, keepdim=True) + r * (G * o).square().sum(-1, keepdim=True)
             gain = 0.0
             if stored_out:
                 delta = delta + (G * o).square().sum(-1, keepdim=True)
@@ -45,8 +49,8 @@ def _sizes(q, k, v, do, scale, keep=None, stored_out=False):
             out[3][b, at, e] += p.T @ G
             # sum_j p^2 (v - o)^2
             var[0][b, :, h] = f * (p.square() @ V.square() - 2 * (p.square() @ V) * o + p.square().sum(-1, keepdim=True) * o.square())
-            var[1][b, :, h] = f * (ds.square() @ K.square() * scale ** 2 + delta * pk.square() + gain * (ds @ K * scale).square())
-            var[2][b, at, e] += f * ((ds.square() + p.square() * delta + gain * ds.square()).T @ Q.square()) * scale ** 2
+            var[1][b, :, h] = f * (ds2 @ K.square() * scale ** 2 + delta * pk.square() + gain * (ds @ K * scale).square())
+            var[2][b, at, e] += f * ((ds2 + p.square() * delta + gain * ds.square()).T @ Q.square()) * scale ** 2
             var[3][b, at, e] += f * ((1 + gain) * p.square()).T @ G.square()
     return out, var
 
@@ -127,3 +131,52 @@ def test_float16_infinite_gradients_stay_where_they_belong(D, Lk):
     assert not torch.isfinite(got[1][0, 33]).any() and not torch.isfinite(got[2]).all() and not torch.isfinite(got[3][..., 5]).any()
     rest = torch.arange(90, device=_dev()) != 33
     assert torch.equal(got[1][:, rest], clean[1][:, rest]) and torch.equal(got[0], clean[0])
+
+
+MANY_ROWS = [(1, 4000, 12, 4, 1, 128, 0), (1, 4000, 12, 4, 1, 64, 4), (1, 1000, 300, 8, 1, 64, 12), (1, 600, 40, 4, 1, 41, 0), (2, 2100, 65, 2, 2, 72, 0), (1, 40, 200, 64, 1, 64, 0),
+             (1, 33, 130, 96, 2, 128, 13), (3, 1111, 1, 2, 1, 32, 0), (1, 2000, 700, 2, 1, 100, 7)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,Lq,Lk,H,E,D,groups", MANY_ROWS)
+def test_many_rows_over_few_keys(dtype, B, Lq, Lk, H, E, D, groups):
+    """dK and dV of few keys: the rows are dealt to several workgroups, and their parts added up."""
+    g = _gen(75)
+    q, k, v, do = (_randn(g, *s, dtype=dtype) for s in ((B, Lq, H, D), (B, Lk, E, D), (B, Lk, E, D), (B, Lq, H, D)))
+    keep = None
+    if groups:
+        keep = torch.rand(B, groups, generator=g, device=_dev()) < 0.6
+        keep[0, 0], keep[0, 1] = True, False
+    want, var = _sizes(q, k, v, do, D ** -0.5, keep)
+    got = _call(q, k, v, do, keep)
+    _check(got, want, var, dtype)
+    if groups:
+        gone = ~keep.repeat_interleave(Lk // groups, 1)
+        assert not got[2][gone].any() and not got[3][gone].any()
+    assert all(torch.equal(a, b) for a, b in zip(_call(q, k, v, do, keep), got))   # bit-reproducible
+
+
+def test_many_rows_over_few_keys_in_graphs():
+    """The parts' memory is the graph's own: two graphs replayed in turn, eager calls between."""
+    B, Lq, Lk, H, E, D, _ = MANY_ROWS[2]
+    shapes = ((B, Lq, H, D), (B, Lk, E, D), (B, Lk, E, D), (B, Lq, H, D))
+    inputs = lambda n: [_randn(_gen(n + 100 * k), *s, dtype=torch.bfloat16) for k, s in enumerate(shapes)]  # noqa: E731
+    static = [inputs(1), inputs(2)]
+    _call(*static[0])
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for s in static:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(_call(*s))
+    for turn in range(3):
+        now = [inputs(10 + 2 * turn + k) for k in range(2)]
+        for n, s in zip(now, static):
+            for a, b in zip(s, n):
+                a.copy_(b)
+        for graph in graphs:
+            graph.replay()
+        eager = [_call(*n) for n in now]
+        torch.cuda.synchronize()
+        for got, want in zip(outs, eager):
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), turn
