@@ -1,11 +1,12 @@
 """-m gpu: calls of the operators on view tokens that programs make now and then: infinities on the way back, gradients of gradients, traced and
 replayed calls, sizes and grids past the first round."""
+import itertools
 import math
 
 import pytest
 import torch
 
-from mvtn_amd import tokens
+from mvtn_amd import _lib, tokens
 
 from gpu_helpers import _dev
 from test_gpu_tokens import _gen, _randn
@@ -271,3 +272,46 @@ def test_a_last_batch_without_objects():
     for B, Lq, Lk, keep in ((0, 4, 6, (0, 3)), (2, 4, 0, (2, 0)), (2, 4, 0, (2, 5)), (0, 4, 0, (0, 0))):
         got = _attention(h(B, Lq, 2, 16), h(B, Lk, 2, 16), h(B, Lk, 2, 16), h(B, Lq, 2, 16), torch.zeros(*keep, device=_dev()))
         assert [tuple(t.shape) for t in got] == [(B, Lq, 2, 16)] * 2 + [(B, Lk, 2, 16)] * 2 and not any(t.any() for t in got)
+
+
+@pytest.mark.parametrize("which", range(3))
+def test_some_leaves_only(which):
+    """Frozen keys, a learned query, cameras alone: the gradients that are asked for are those of the full backward, bit by bit."""
+    call, inputs = _operators()[which]
+    leaves = [t.detach().requires_grad_() for t in inputs]
+    out = call(*leaves)
+    up = torch.randn_like(out)
+    full = torch.autograd.grad(out, leaves, up)
+    for wanted in itertools.product((False, True), repeat=len(inputs)):
+        if not any(wanted):
+            continue
+        some = [t.detach().requires_grad_(w) for t, w in zip(inputs, wanted)]
+        again = call(*some)
+        assert torch.equal(again, out)
+        got = torch.autograd.grad(again, [t for t, w in zip(some, wanted) if w], up)
+        assert all(torch.equal(a, b) for a, b in zip(got, [g for g, w in zip(full, wanted) if w])), wanted
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,Lq,Lk,H,E,D", [(2, 150, 300, 4, 2, 64), (1, 2, 3000, 4, 2, 128), (2, 40, 50, 2, 2, 40)])
+def test_the_c_abi_without_the_outputs_rest(dtype, B, Lq, Lk, H, E, D):
+    """mvr_attend_tokens_forward and _backward, for programs that keep out and lse alone: the same output, gradients that carry out's rounding too."""
+    from test_gpu_tokens_accuracy import _check, _sizes
+    g = _gen(96)
+    q, k, v, do = (_randn(g, *s, dtype=dtype) for s in ((B, Lq, H, D), (B, Lk, E, D), (B, Lk, E, D), (B, Lq, H, D)))
+    lib, p = _lib.load(), lambda t: t.data_ptr()  # noqa: E731
+    a = _lib.AttendParams(B, Lq, Lk, H, E, D, {torch.float16: 1, torch.bfloat16: 2}[dtype], 0)
+    a.scale = D ** -0.5
+    for t, s in ((q, a.q_stride), (k, a.k_stride), (v, a.v_stride), (do, a.grad_stride)):
+        s[:] = t.stride()[:3]
+    room = [torch.empty(max(lib.mvr_attend_tokens_workspace_bytes(a, n), 1), dtype=torch.uint8, device=_dev()) for n in (0, 1)]
+    out, lse = torch.empty_like(q), torch.empty(B, H, Lq, device=_dev())
+    grads = [torch.empty_like(t) for t in (q, k, v)]
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.mvr_attend_tokens_forward(a, p(q), p(k), p(v), None, p(out), p(lse), p(room[0]), room[0].numel(), stream) == 0
+    assert lib.mvr_attend_tokens_backward(a, p(q), p(k), p(v), None, p(out), p(lse), p(do), *map(p, grads), p(room[1]), room[1].numel(), stream) == 0
+    want, var = _sizes(q, k, v, do, D ** -0.5, stored_out=True)
+    _check([out] + grads, want, var, dtype)
+    assert torch.equal(out, tokens.attend_tokens(q, k, v))
+    scores = torch.einsum("bqehd,bked->behqk", q.double().view(B, Lq, E, H // E, D), k.double()) * D ** -0.5
+    assert torch.allclose(lse.double(), scores.logsumexp(-1).reshape(B, H, Lq) / math.log(2), rtol=0, atol=2.0 ** -16)   # (of numbers below 16: 2^-20 each of score and sum)
