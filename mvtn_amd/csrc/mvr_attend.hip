@@ -713,7 +713,7 @@ __global__ __launch_bounds__(kBlock, 2) void k_attend_dq(AttArgs a) {
   walk_tiles(a, b, first, last, MVR_ATT_KV, step);
   if (FINE && writes) a.delta[be * a.rows + c.row] = delta;
   if (c.live) {
-    const float back = kNarrow<T> ? __builtin_amdgcn_exp2f(-power) : 1.0f;
+    const float back = kNarrow<T> ? __builtin_ldexpf(1.0f, -(int)power) : 1.0f;
     if constexpr (SPLIT) store_column<float, DP>(a.part + ((split * (int64_t)a.B * a.E + be) * a.rows + c.row) * a.D, a.D, dq, back);
     else store_column<T, DP>((T *)a.dq + (((int64_t)b * a.Lq + c.i) * a.H + e * a.G + c.g) * a.D, a.D, dq, a.scale * back);
   }
