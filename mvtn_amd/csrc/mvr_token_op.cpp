@@ -237,8 +237,7 @@ Tensor rotate_tokens(const Tensor &x, const Tensor &positions, Doubles turns, In
   check_rotary(x, positions, turns, sections, interleaved);
   no_forward_mode({&x, &positions});
   same_device(x, {&positions});
-  MVR_OP("rotate_forward", rotate_forward_gpu);
-  return op.call(rows_packed(x), positions.to(at::kFloat).expand_symint({x.sym_size(0), x.sym_size(1), (int64_t)sections.size()}), turns, sections, interleaved);
+  return rotate_forward_autograd(rows_packed(x), positions.to(at::kFloat).expand_symint({x.sym_size(0), x.sym_size(1), (int64_t)sections.size()}), turns, sections, interleaved);
 }
 
 // ---- attention ---------------------------------------------------------------------------------------------------------
@@ -380,8 +379,7 @@ Tensor attend_tokens(const Tensor &q, const Tensor &k, const Tensor &v, const Ma
   no_forward_mode({&q, &k, &v});
   same_device(q, {&k, &v, &keep});
   if (keep.defined()) keep = (keep.scalar_type() == at::kBool || keep.scalar_type() == at::kByte ? keep : keep.ne(0)).contiguous();
-  MVR_OP("attend_forward", attend_forward_gpu);
-  return op.call(rows_packed(q), rows_packed(k), rows_packed(v), some(keep), scale);
+  return attend_forward_autograd(rows_packed(q), rows_packed(k), rows_packed(v), some(keep), scale);
 }
 
 // ---- norms around a block ----------------------------------------------------------------------------------------------
@@ -569,8 +567,7 @@ Two add_norm_tokens(MVR_NORM_INPUTS) {
   no_forward_mode({&residual, &branch, &weight, &bias, &post, &gate});
   same_device(residual, {&branch, &weight, &bias, &post, &gate, &draws});
   if (draws.defined()) draws = draws.to(at::kFloat).contiguous();
-  MVR_OP("add_norm_forward", norm_forward_gpu);
-  return op.call(residual, branch, weight, bias_, post_, gate_, some(draws), number, layer, eps);
+  return norm_forward_autograd(residual, branch, weight, bias_, post_, gate_, some(draws), number, layer, eps);
 }
 
 }  // namespace
