@@ -3,7 +3,7 @@
 //   dV = P^T dO,  dS = P (dO v^T - delta),  delta = rowsum(dO O),  dQ = scale dS k,  dK = scale dS^T q
 // One pass over the keys with the running maximum and sum; nothing of size queries x keys is ever stored: the backward recomputes the
 // probabilities from q, k and lse.  Sums, maxima and exponentials are 32 bits wide; P and dS are rounded to the tensors' type where they
-// enter a matrix instruction: half a step of the type relative to each, as of the inputs, and not where few keys make it count (FINE, at k_attend_dq).
+// enter a matrix instruction: half a step of the type relative to each, as of the inputs, and not where few keys make it count (FINE, at k_attend).
 // The forward's P lies in [0, 2^8], as its maximum may lag.  In float16, whose step stops shrinking at 2^-14, P and dS enter times a power of two
 // that brings them to the top of its range, and the 32-bit sums are divided by it (at kLift).
 //
@@ -423,7 +423,7 @@ __device__ __forceinline__ void mask_scores(f32x16 &s, unsigned long long m, int
 }
 
 // The running maximum only has to keep exponentials in range: it follows the scores when one exceeds it by more than kSlack (powers of two),
-// and only then are sum and output rescaled.  Probabilities then reach 2^8, far from any type's limit, and their rounding is relative.
+// and only then are sum and output rescaled.  Probabilities then reach 2^8 (2^15 in float16, with kLift: half its largest number), and their rounding is relative.
 // (Following every new maximum, one of a wave's 64 columns has one in four tiles of five, at 68 multiplications each.)
 constexpr float kSlack = 8.0f;
 
